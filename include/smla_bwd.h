@@ -159,6 +159,78 @@ typedef struct smla_fwd_params {
 size_t smla_fwd_workspace_size(const smla_fwd_params* p, size_t budget_bytes);
 int smla_fwd_run(const smla_fwd_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- serving: a paged cache of kv rows in 8 bits ---------------------------------------------------------
+ * (No counterpart in the reference, whose operators read kv as one bf16 tensor.)
+ * The cache: values, e4m3 [n_pages, page_size, 576], and scales, fp32 [n_pages]: what is stored is value * scale of its page.  A scale
+ * is a power of two.  page_size: 16, 32, 64 or 128.  A slot is page * page_size + row.  A block table i32 [n_requests, max_pages] names the
+ * pages of each request's tokens in their order; page_size * max_pages may be up to 2^30, n_pages * page_size less than 2^31. */
+
+/* Tables of one step, made on the GPU from the requests' lengths.  With have = pages of kv_len tokens:
+ *   new_len[i] < 0: the request ends, its pages go back onto the stack of free pages (in order of requests and pages), kv_len 0;
+ *   else new_len[i] tokens are appended: pages for them are taken from the top of the stack and entered into the block table behind the
+ *   request's `have`.  Requests are served in order.  One that does not fit - the stack has not enough pages, kv_len + new_len is more
+ *   than max_pages * page_size, its tokens' rows would end behind max_tokens, kv_len < 0 - gets none (admitted 0, kv_len as it
+ *   was), and so does every later one that needs a page once the stack had too few.
+ * Token rows are packed in order of requests, new_len[i] of them for each (whether or not it is admitted):
+ *   slots i32 [max_tokens]           slot of the token, -1 for rows of requests not admitted and behind the last
+ *   query_meta i32 [max_tokens][4]   {request, its tokens after the step, the token's position, topk}; zeros where the slot is -1
+ * free_pages [n_free] (the stack: entries below *free_count are free) and block_table are updated in place; kv_len_out, free_count_out
+ * and admitted (tokens) are written; kv_len, new_len and free_count are not changed, so a call made twice does the same again.
+ * At most 8192 requests.  max_tokens may be 0 (a step that only ends requests); slots and query_meta may be null then. */
+typedef struct smla_cache_plan_params {
+    const int32_t* kv_len;      /* [n_requests] tokens in the cache */
+    const int32_t* new_len;     /* [n_requests] */
+    const int32_t* free_count;  /* [1] */
+    int32_t* block_table;       /* [n_requests, max_pages] */
+    int32_t* free_pages;        /* [n_free] */
+    int32_t* slots;             /* [max_tokens] */
+    int32_t* query_meta;        /* [max_tokens, 4], 16-byte aligned */
+    int32_t* kv_len_out;        /* [n_requests] */
+    int32_t* free_count_out;    /* [1] */
+    int32_t* admitted;          /* [n_requests] */
+    int32_t n_requests, max_pages, n_free, page_size, max_tokens, topk;
+} smla_cache_plan_params;
+int smla_cache_plan(const smla_cache_plan_params* p, void* stream);
+
+/* Writes rows into the cache.  kv: bf16 [n_rows, 576] with kv_stride elements from row to row (a multiple of 8), slots i32 [n_rows]; rows
+ * whose slot is outside the cache are left out, of several rows with one slot the last one is kept.  A page whose row 0 is among the
+ * slots starts anew: its scale becomes the smallest power of two (2^-100 at least) that holds the call's rows in the page, and its
+ * other rows stay as they are, void.  Any other page's scale grows to that where it is smaller, and the rows it keeps are brought over to the
+ * new scale.  Rows are rounded to the nearest; a number that is not finite is stored as a NaN and does not count for the scale.
+ * `workspace` (256-byte aligned, smla_cache_append_workspace_size() bytes, may be null where that is 0). */
+typedef struct smla_cache_append_params {
+    const void* kv;
+    const int32_t* slots;
+    void* values;
+    float* scales;
+    int64_t kv_stride;
+    int32_t n_rows, n_pages, page_size;
+} smla_cache_append_params;
+size_t smla_cache_append_workspace_size(int32_t n_rows);
+int smla_cache_append(const smla_cache_append_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* smla_fwd_run over the cache.  `query_meta` as smla_cache_plan writes it: {request, its tokens in the cache, position for the causal
+ * rule, top-k slots in use}; index values are positions in the request, valid in [0, tokens), and with `causal` != 0 only up to the
+ * query's position.  A slot whose page number is outside the cache takes no part.  Only a scale's exponent is used, and one below 2^-100
+ * counts as 2^-100.  Queries are split into two 8-bit numbers, exact for what is within 2^-10 of a row's largest magnitude; a row of q that
+ * holds an infinity gives NaN. */
+typedef struct smla_fwd_cached_params {
+    const void* q;              /* bf16 [s_q, h_q, 576] */
+    const void* values;
+    const float* scales;
+    const int32_t* block_table;
+    const int32_t* indices;     /* i32 [s_q, topk] */
+    const int32_t* query_meta;  /* i32 [s_q, 4], 16-byte aligned */
+    void* o;                    /* bf16 [s_q, h_q, 512] (0 for a query without a valid slot) */
+    float* lse;                 /* f32 [s_q, h_q] (+inf for a query without a valid slot) */
+    int32_t s_q, h_q, topk, n_pages, page_size, n_requests, max_pages;
+    float sm_scale;             /* <= 0 selects 1/sqrt(576) */
+    int32_t causal;
+    int32_t lse_is_base2;
+} smla_fwd_cached_params;
+size_t smla_fwd_cached_workspace_size(const smla_fwd_cached_params* p, size_t budget_bytes);
+int smla_fwd_cached_run(const smla_fwd_cached_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Delta only: delta[s_q, h_q] = sum_j O[.., j] * dO[.., j]   (reference: launch_preprocess_delta). */
 int smla_bwd_delta(const void* O, const void* dO, float* delta, int32_t s_q, int32_t h_q, void* stream);
 

@@ -21,7 +21,7 @@ setup(
             name="mla_bwd_cuda",
             sources=[os.path.join(CSRC, "mla_bwd_ext.cpp"), os.path.join(CSRC, "smla_api.cu")],
             include_dirs=[os.path.join(ROOT, "include")],
-            depends=[os.path.join(CSRC, h) for h in ("sm100_ptx.cuh", "smla_kernels.cuh", "smla_index_inverse.cuh")]
+            depends=[os.path.join(CSRC, h) for h in ("sm100_ptx.cuh", "smla_kernels.cuh", "smla_index_inverse.cuh", "smla_cache.cuh", "smla_fwd_cached.cuh")]
             + [os.path.join("include", "smla_bwd.h")],
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],

@@ -23,7 +23,7 @@ HOST_HEADER = os.path.join(ROOT, "include", "smla_bwd.h")
 HOST_DELTA = os.path.join(CSRC, "smla_host_delta.h")
 
 SOURCES = ["smla_api.cu"]
-HEADERS = ["sm100_ptx.cuh", "smla_kernels.cuh", "smla_index_inverse.cuh"]
+HEADERS = ["sm100_ptx.cuh", "smla_kernels.cuh", "smla_index_inverse.cuh", "smla_cache.cuh", "smla_fwd_cached.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -16,6 +16,8 @@
 #include "../../include/smla_bwd.h"
 #include "smla_kernels.cuh"
 #include "smla_index_inverse.cuh"
+#include "smla_cache.cuh"
+#include "smla_fwd_cached.cuh"
 
 namespace {
 
@@ -532,15 +534,8 @@ bool fwd_plan_for_workspace(const smla_fwd_params* p, size_t ws_bytes, FwdPlan* 
     return make_fwd_plan(p, ws_bytes, pl) && pl->total <= ws_bytes;
 }
 
-template <int HP>
-int launch_fwd_chain(const smla_fwd_params* p, const FwdPlan& pl, uint8_t* ws, cudaStream_t st) {
-    using namespace smla;
-    if (!bind_context()) return SMLA_ERR_LAUNCH;
-    CUtensorMap tm_q;
-    if (!make_map_2d(&tm_q, p->q, kDQK, uint64_t(p->s_q) * p->h_q, kDQK * 2, 64, HP / 2)) return SMLA_ERR_LAUNCH;
-    static std::atomic<bool> attr_done[kMaxDevices];
-    if (!once_per_device(attr_done, [] { return set_smem(smla_fwd_kernel<HP>, ff::kSmemBytes); })) return SMLA_ERR_LAUNCH;
-
+KParams fwd_kparams(const smla_fwd_params* p, const FwdPlan& pl, uint8_t* ws) {
+    using smla::kDQK;
     KParams kp{};
     kp.kv = reinterpret_cast<const __nv_bfloat16*>(p->kv);
     kp.indices = p->indices;
@@ -565,25 +560,94 @@ int launch_fwd_chain(const smla_fwd_params* p, const FwdPlan& pl, uint8_t* ws, c
     kp.wait_limit = g_wait_limit.load();
     kp.q0 = 0;
     kp.nq = p->s_q;
-    const int pairs = resident_pairs(smla_fwd_kernel<HP>, ff::kThreads, ff::kSmemBytes);
+    return kp;
+}
+
+// The forward's kernels around the main one, which `main` launches with the grid it is given: `pairs` clusters of it are resident.
+template <int HP, typename F>
+int launch_fwd_kernels(KParams& kp, const FwdPlan& pl, uint8_t* ws, cudaStream_t st, int pairs, F main) {
+    using namespace smla;
     if (pairs <= 0) return SMLA_ERR_LAUNCH;
     const int clusters = std::max(1, std::min(pairs, pl.clusters));
     const int q_tiles = pl.topk_pad / kWorkTileKeys;
-    if (at_most_a_tile_each(p->s_q, q_tiles, clusters))
-        kp.every_slot = p->topk;
+    if (at_most_a_tile_each(kp.s_q, q_tiles, clusters))
+        kp.every_slot = kp.topk;
     else
-        launch(smla_prep_kernel, p->s_q, kPrepThreads, 0, st, true, 1, static_cast<const uint4*>(nullptr), static_cast<const uint4*>(nullptr),
+        launch(smla_prep_kernel, kp.s_q, kPrepThreads, 0, st, true, 1, static_cast<const uint4*>(nullptr), static_cast<const uint4*>(nullptr),
                static_cast<float*>(nullptr), reinterpret_cast<int*>(ws + pl.used_off), 1, kp);
-    launch(smla_fwd_kernel<HP>, 2 * clusters, ff::kThreads, ff::kSmemBytes, st, true, 1, tm_q, kp);
+    main(2 * clusters);
     if (clusters > 1 && (!kp.every_slot || q_tiles > 1)) {
-        const int items = p->s_q < clusters ? p->s_q : clusters - 1;
-        const int grid = items * ((p->h_q + 31) / 32 * (1024 / kCombineThreads));
+        const int items = kp.s_q < clusters ? kp.s_q : clusters - 1;
+        const int grid = items * ((kp.h_q + 31) / 32 * (1024 / kCombineThreads));
         // (as many queries as clusters, of about equal length: a query lies in two ranges, seldom in three)
-        const bool two_parts = kp.every_slot ? q_tiles <= 2 : p->s_q >= clusters;
+        const bool two_parts = kp.every_slot ? q_tiles <= 2 : kp.s_q >= clusters;
         if (two_parts) launch(smla_fwd_combine_kernel<2>, grid, kCombineThreads, 0, st, true, 1, kp, clusters, HP);
         else launch(smla_fwd_combine_kernel<4>, grid, kCombineThreads, 0, st, true, 1, kp, clusters, HP);
     }
     return cudaGetLastError() == cudaSuccess ? SMLA_OK : SMLA_ERR_LAUNCH;
+}
+
+template <int HP>
+int launch_fwd_chain(const smla_fwd_params* p, const FwdPlan& pl, uint8_t* ws, cudaStream_t st) {
+    using namespace smla;
+    if (!bind_context()) return SMLA_ERR_LAUNCH;
+    CUtensorMap tm_q;
+    if (!make_map_2d(&tm_q, p->q, kDQK, uint64_t(p->s_q) * p->h_q, kDQK * 2, 64, HP / 2)) return SMLA_ERR_LAUNCH;
+    static std::atomic<bool> attr_done[kMaxDevices];
+    if (!once_per_device(attr_done, [] { return set_smem(smla_fwd_kernel<HP>, ff::kSmemBytes); })) return SMLA_ERR_LAUNCH;
+
+    KParams kp = fwd_kparams(p, pl, ws);
+    return launch_fwd_kernels<HP>(kp, pl, ws, st, resident_pairs(smla_fwd_kernel<HP>, ff::kThreads, ff::kSmemBytes), [&](int grid) {
+        launch(smla_fwd_kernel<HP>, grid, ff::kThreads, ff::kSmemBytes, st, true, 1, tm_q, kp);
+    });
+}
+
+// ---- forward over the paged cache --------------------------------------------------------------------------
+bool page_size_ok(int32_t page_size) { return page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128; }
+int log2_of(int32_t power) { return 31 - __builtin_clz(static_cast<unsigned>(power)); }
+bool cache_shape_ok(int32_t n_pages, int32_t page_size) {
+    return n_pages > 0 && page_size_ok(page_size) && static_cast<long long>(n_pages) * page_size <= INT_MAX;
+}
+constexpr long long kMaxRequestTokens = 1LL << 30;
+
+// The part of the parameters that the forward's workspace goes by, as the forward has it.
+bool cached_as_fwd(const smla_fwd_cached_params* p, smla_fwd_params* f) {
+    if (!p || !cache_shape_ok(p->n_pages, p->page_size) || p->n_requests <= 0 || p->max_pages <= 0) return false;
+    if (p->n_requests > INT_MAX / 2 || static_cast<long long>(p->max_pages) * p->page_size > kMaxRequestTokens) return false;
+    *f = smla_fwd_params{};
+    f->q = p->q;
+    f->indices = p->indices;
+    f->o = p->o;
+    f->lse = p->lse;
+    f->s_q = p->s_q;
+    f->s_kv = INT_MAX;          // (the slot counts' rule adds the request's number to an index)
+    f->h_q = p->h_q;
+    f->topk = p->topk;
+    f->sm_scale = p->sm_scale;
+    f->q_start_index_s = p->causal ? 0 : SMLA_NO_CAUSAL;
+    f->lse_is_base2 = p->lse_is_base2;
+    f->query_meta = p->query_meta;
+    return check_fwd_params(f);
+}
+
+template <int HP>
+int launch_fwd_cached_chain(const smla_fwd_cached_params* p, const smla_fwd_params* f, const FwdPlan& pl, uint8_t* ws, cudaStream_t st) {
+    using namespace smla;
+    static std::atomic<bool> attr_done[kMaxDevices];
+    if (!once_per_device(attr_done, [] { return set_smem(smla_fwd_cached_kernel<HP>, fc::kSmemBytes); })) return SMLA_ERR_LAUNCH;
+    KParams kp = fwd_kparams(f, pl, ws);
+    CacheView c{};
+    c.values = static_cast<const uint8_t*>(p->values);
+    c.scales = p->scales;
+    c.table = p->block_table;
+    c.q = static_cast<const __nv_bfloat16*>(p->q);
+    c.n_pages = p->n_pages;
+    c.page_shift = log2_of(p->page_size);
+    c.n_req = p->n_requests;
+    c.max_pages = p->max_pages;
+    return launch_fwd_kernels<HP>(kp, pl, ws, st, resident_pairs(smla_fwd_cached_kernel<HP>, fc::kThreads, fc::kSmemBytes), [&](int grid) {
+        launch(smla_fwd_cached_kernel<HP>, grid, fc::kThreads, fc::kSmemBytes, st, true, 1, kp, c);
+    });
 }
 
 // ---- workspace that lives in the library image (smla_bwd_run_noalloc) -----------------------------------
@@ -857,6 +921,98 @@ int smla_fwd_run(const smla_fwd_params* p, void* workspace, size_t workspace_byt
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     return pl.h_pad == 64 ? launch_fwd_chain<64>(p, pl, ws, st) : launch_fwd_chain<128>(p, pl, ws, st);
+}
+
+size_t smla_fwd_cached_workspace_size(const smla_fwd_cached_params* p, size_t budget_bytes) {
+    smla_fwd_params f;
+    return cached_as_fwd(p, &f) ? smla_fwd_workspace_size(&f, budget_bytes) : 0;
+}
+
+int smla_fwd_cached_run(const smla_fwd_cached_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+    g_last_launches = 0;
+    smla_fwd_params f;
+    if (!cached_as_fwd(p, &f) || !workspace) return SMLA_ERR_BAD_ARG;
+    if (!p->q || !p->values || !p->scales || !p->block_table || !p->indices || !p->query_meta || !p->o || !p->lse) return SMLA_ERR_BAD_ARG;
+    if (!aligned16(p->q) || !aligned16(p->values) || !aligned16(p->o) || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1)))
+        return SMLA_ERR_BAD_ARG;
+    FwdPlan pl;
+    if (!fwd_plan_for_workspace(&f, workspace_bytes, &pl)) return SMLA_ERR_WORKSPACE;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    return pl.h_pad == 64 ? launch_fwd_cached_chain<64>(p, &f, pl, ws, st) : launch_fwd_cached_chain<128>(p, &f, pl, ws, st);
+}
+
+int smla_cache_plan(const smla_cache_plan_params* p, void* stream) {
+    using namespace smla;
+    g_last_launches = 0;
+    if (!p || !p->kv_len || !p->new_len || !p->free_count || !p->block_table || !p->free_pages || !p->kv_len_out || !p->free_count_out || !p->admitted)
+        return SMLA_ERR_BAD_ARG;
+    if (p->max_tokens && (!p->slots || !p->query_meta || !aligned16(p->query_meta))) return SMLA_ERR_BAD_ARG;
+    if (p->n_requests <= 0 || p->n_requests > kMaxCacheRequests || p->max_pages <= 0 || p->n_free <= 0 || !page_size_ok(p->page_size) ||
+        p->max_tokens < 0 || p->max_tokens >= (1 << 30) || p->topk < 0)
+        return SMLA_ERR_BAD_ARG;
+    if (static_cast<long long>(p->max_pages) * p->page_size > kMaxRequestTokens ||
+        static_cast<long long>(p->n_requests) * p->max_pages + p->n_free > INT_MAX)
+        return SMLA_ERR_BAD_ARG;
+    const int smem = (4 * p->n_requests + 3) * 4;
+    static std::atomic<bool> attr_done[kMaxDevices];
+    if (!once_per_device(attr_done, [] { return set_smem(smla_cache_plan_kernel, (4 * kMaxCacheRequests + 3) * 4); })) return SMLA_ERR_LAUNCH;
+    CachePlanArgs a{};
+    a.kv_len = p->kv_len;
+    a.new_len = p->new_len;
+    a.free_count = p->free_count;
+    a.table = p->block_table;
+    a.free_pages = p->free_pages;
+    a.slots = p->slots;
+    a.kv_len_out = p->kv_len_out;
+    a.free_count_out = p->free_count_out;
+    a.admitted = p->admitted;
+    a.meta = reinterpret_cast<int4*>(p->query_meta);
+    a.n_req = p->n_requests;
+    a.max_pages = p->max_pages;
+    a.n_free = p->n_free;
+    a.page_shift = log2_of(p->page_size);
+    a.max_tokens = p->max_tokens;
+    a.topk = p->topk;
+    const int blocks = std::max(1, std::min(kSmCount, (p->max_tokens + kCachePlanThreads - 1) / kCachePlanThreads));
+    launch(smla_cache_plan_kernel, blocks, kCachePlanThreads, smem, reinterpret_cast<cudaStream_t>(stream), true, 1, a);
+    return cudaGetLastError() == cudaSuccess ? SMLA_OK : SMLA_ERR_LAUNCH;
+}
+
+size_t smla_cache_append_workspace_size(int32_t n_rows) {
+    if (n_rows <= smla::kAppendDirect) return 0;
+    return align_up(size_t(n_rows) * sizeof(int2), kAlign) + smla::kAppendMaxLists * sizeof(int);
+}
+
+int smla_cache_append(const smla_cache_append_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace smla;
+    g_last_launches = 0;
+    if (!p || !p->kv || !p->slots || !p->values || !p->scales || !aligned16(p->kv) || !aligned16(p->values)) return SMLA_ERR_BAD_ARG;
+    if (p->n_rows <= 0 || !cache_shape_ok(p->n_pages, p->page_size) || p->kv_stride < 0 || p->kv_stride % 8 != 0) return SMLA_ERR_BAD_ARG;
+    const size_t need = smla_cache_append_workspace_size(p->n_rows);
+    if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1)))) return SMLA_ERR_BAD_ARG;
+    if (workspace_bytes < need) return SMLA_ERR_WORKSPACE;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    CacheAppendArgs a{};
+    a.kv = static_cast<const __nv_bfloat16*>(p->kv);
+    a.kv_stride = p->kv_stride;
+    a.values = static_cast<uint8_t*>(p->values);
+    a.scales = p->scales;
+    a.slots = p->slots;
+    a.n_rows = p->n_rows;
+    a.n_pages = p->n_pages;
+    a.page_shift = log2_of(p->page_size);
+    if (!need) {
+        launch(smla_cache_append_kernel, p->n_rows, kAppendThreads, 0, st, true, 1, a);
+    } else {
+        a.list_len = std::max(kAppendListLen, (p->n_rows + kAppendMaxLists - 1) / kAppendMaxLists);
+        a.n_lists = (p->n_rows + a.list_len - 1) / a.list_len;
+        a.runs = static_cast<int2*>(workspace);
+        a.counts = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + align_up(size_t(p->n_rows) * sizeof(int2), kAlign));
+        launch(smla_cache_runs_kernel, a.n_lists, 1024, 0, st, true, 1, a);
+        launch(smla_cache_append_listed_kernel, kSmCount * 8, kAppendThreads, 0, st, true, 1, a);
+    }
+    return cudaGetLastError() == cudaSuccess ? SMLA_OK : SMLA_ERR_LAUNCH;
 }
 
 int smla_bwd_delta(const void* O, const void* dO, float* delta, int32_t s_q, int32_t h_q, void* stream) {

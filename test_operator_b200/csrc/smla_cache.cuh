@@ -1,0 +1,384 @@
+// Device kernels around the paged cache of kv rows in 8 bits: the tables of a serving step (pages for new tokens, slot map, query
+// table) and the write of new rows.  The attention that reads the cache is in smla_fwd_cached.cuh.
+//
+// The cache: values e4m3 [n_pages][page rows][576], scales fp32 [n_pages].  A page's rows share one scale, a power of two, so that going
+// over to a larger scale moves exponents only (a number rounds again only where it becomes subnormal), and so that a stored number
+// times its scale is a bf16 number exactly.  A slot is page * page rows + row.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "smla_kernels.cuh"
+
+namespace smla {
+
+constexpr int kMinScaleExp = -100;          // rows are stored with a scale of 2^-100 at least
+constexpr int kMaxPageRows = 128;
+
+// The smallest e >= kMinScaleExp with amax <= 448 * 2^e (448: the largest e4m3 number, 1.75 * 2^8), for a finite amax >= 0.
+__device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
+    const int e = static_cast<int>(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return max(e, kMinScaleExp);
+}
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+
+// Two numbers -> e4m3, nearest even, `lo` in the low byte.  What is beyond 448 becomes 448, a NaN stays one.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// =============================================================================================
+// Tables of a step.
+//
+// Every block adds up the requests' pages and tokens itself (8 bytes a request out of L2) and then takes its share of the tokens and
+// of the pages that change hands, so one launch does it, with no prefix sums in memory.  That needs no order between the blocks: what is
+// read (free_pages below free_count, the block table's entries of pages that requests had before the call) is not written by any
+// of them.  A page that is given back and taken again in the same call is looked up in the row of the request that gives it.
+// Bound by latency: a launch, two dependent loads and three block sums.
+// =============================================================================================
+struct CachePlanArgs {
+    const int *kv_len, *new_len, *free_count;
+    int *table, *free_pages;
+    int *slots, *kv_len_out, *free_count_out, *admitted;
+    int4* meta;
+    int n_req, max_pages, n_free, page_shift, max_tokens, topk;
+};
+constexpr int kCachePlanThreads = 512;
+constexpr int kMaxCacheRequests = 8192;
+
+// The largest i < n with a[i] <= x, for a[0] = 0 <= x and a[] not decreasing.
+__device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// Sum of one value per thread over the lower-numbered threads, not above `cap`, for values of 0 .. cap and a cap below 2^30; *total: over all.
+__device__ __forceinline__ int block_exclusive_capped_sum(int v, int cap, int* warp_sums, int* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl = min(incl + up, cap);
+    }
+    const int left = __shfl_up_sync(0xffffffffu, incl, 1);
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < n_warps; ++w) {
+        if (w == warp) before = all;
+        all = min(all + warp_sums[w], cap);
+    }
+    __syncthreads();
+    *total = all;
+    return lane ? min(before + left, cap) : before;
+}
+
+__global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(const CachePlanArgs a) {
+    extern __shared__ int plan_smem[];
+    __shared__ int warp_sums[kCachePlanThreads / 32];
+    int* first = plan_smem;                       // [n_req + 1] tokens of the requests before, at most max_tokens + 1
+    int* len = first + a.n_req + 1;               // [n_req] kv_len, ~kv_len of a request that gets no row
+    int* needx = len + a.n_req;                   // [n_req + 1] new pages asked for by the requests before
+    int* backx = needx + a.n_req + 1;             // [n_req + 1] pages given back by the requests before
+    pdl_wait();
+    pdl_trigger();
+    const int page = 1 << a.page_shift, cap = a.max_tokens + 1;
+    const int n_free = min(max(__ldg(a.free_count), 0), a.n_free);
+    const int per = (a.n_req + kCachePlanThreads - 1) / kCachePlanThreads;
+    const int i0 = min(static_cast<int>(threadIdx.x) * per, a.n_req), i1 = min(i0 + per, a.n_req);
+    const int room = a.max_pages << a.page_shift;                      // (below 2^31: checked on the host)
+    auto length = [&](int i) { return min(max(__ldg(a.kv_len + i), 0), room); };
+    auto pages_of = [&](int tokens) { return (tokens + page - 1) >> a.page_shift; };
+    int back = 0, tokens = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int n = __ldg(a.new_len + i);
+        if (n < 0) back += pages_of(length(i));
+        else tokens = min(tokens + min(n, cap), cap);
+    }
+    int n_back, n_tokens, n_need, n_taken;
+    const int back0 = block_exclusive_sum(back, warp_sums, &n_back);
+    const int first0 = block_exclusive_capped_sum(tokens, cap, warp_sums, &n_tokens);
+    // what request i asks for, given the tokens before it; -1: it cannot have its rows whatever is free
+    auto need_of = [&](int i, int n, int before) {
+        const int old = __ldg(a.kv_len + i);
+        if (n < 0 || old < 0 || old > room || n > room - old || before + min(n, cap) > a.max_tokens) return -1;
+        return pages_of(old + n) - pages_of(old);
+    };
+    int need = 0;
+    for (int i = i0, f = first0; i < i1; ++i) {
+        const int n = __ldg(a.new_len + i);
+        need += max(need_of(i, n, f), 0);
+        f = min(f + min(max(n, 0), cap), cap);
+    }
+    const int need0 = block_exclusive_sum(need, warp_sums, &n_need);
+    const int stack = n_free + n_back;
+    int taken = 0;
+    for (int i = i0, f = first0, u = need0, b = back0; i < i1; ++i) {
+        const int n = __ldg(a.new_len + i), old = length(i), want = need_of(i, n, f);
+        const bool granted = want >= 0 && (want == 0 || u + want <= stack);
+        first[i] = f;
+        len[i] = granted ? old : ~old;
+        needx[i] = u;
+        backx[i] = b;
+        if (blockIdx.x == 0) {
+            a.kv_len_out[i] = n < 0 ? 0 : granted ? old + n : __ldg(a.kv_len + i);
+            a.admitted[i] = granted ? n : 0;
+        }
+        f = min(f + min(max(n, 0), cap), cap);
+        u += max(want, 0);
+        if (granted) taken += want;
+        if (n < 0) b += pages_of(old);
+    }
+    if (threadIdx.x == 0) first[a.n_req] = n_tokens;
+    block_exclusive_sum(taken, warp_sums, &n_taken);           // (its barriers: the tables are whole)
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.free_count_out = min(stack - n_taken, a.n_free);
+    // place s of the stack of free pages, the pages given back on top
+    auto stacked = [&](int s) {
+        if (s < n_free) return __ldg(a.free_pages + s);
+        const int v = s - n_free, i = last_not_above(backx, a.n_req, v);
+        return __ldg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
+    };
+    const int at = blockIdx.x * kCachePlanThreads + threadIdx.x, step = gridDim.x * kCachePlanThreads;
+    for (int t = at; t < a.max_tokens; t += step) {
+        int slot = -1;
+        int4 m = make_int4(0, 0, 0, 0);
+        if (t < n_tokens) {
+            const int i = last_not_above(first, a.n_req, t), old = len[i];
+            if (old >= 0) {
+                const int pos = old + t - first[i], k = pos >> a.page_shift, have = pages_of(old);
+                const int pg = k < have ? __ldg(a.table + static_cast<size_t>(i) * a.max_pages + k) : stacked(stack - 1 - (needx[i] + k - have));
+                slot = pg * page + (pos & (page - 1));
+                m = make_int4(i, old + (first[i + 1] - first[i]), pos, a.topk);
+            }
+        }
+        a.slots[t] = slot;
+        a.meta[t] = m;
+    }
+    for (int u = at; u < n_taken; u += step) {
+        const int i = last_not_above(needx, a.n_req, u);
+        a.table[static_cast<size_t>(i) * a.max_pages + pages_of(len[i]) + (u - needx[i])] = stacked(stack - 1 - u);
+    }
+    for (int v = at; v < n_back && n_free + v < a.n_free; v += step) {
+        const int i = last_not_above(backx, a.n_req, v);
+        a.free_pages[n_free + v] = __ldg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
+    }
+}
+
+// =============================================================================================
+// New rows into the cache.
+//
+// One block per page that the call names: it finds all rows of the call that go to the page, their largest finite magnitude, the page's
+// scale, and writes.  Rows kept by a page whose scale grows are brought over to the new scale in the same block.
+// The first row of a run (neighbours in the call that name one page) speaks for the run; a page may come up in several runs, whose
+// first one does the work for all.  Up to kAppendDirect rows every row has a block, which looks through the whole slot map; beyond that
+// a first kernel lists the runs, and the blocks go through the list.
+// Bound by HBM (1152 bytes read and 576 written a row) for prompts, by latency for the rows of a decoding step.
+// =============================================================================================
+struct CacheAppendArgs {
+    const __nv_bfloat16* kv;
+    long long kv_stride;          // elements from row to row
+    uint8_t* values;
+    float* scales;
+    const int* slots;
+    int n_rows, n_pages, page_shift;
+    int2* runs;                   // [lists][list_len] {page, first row}
+    int* counts;                  // [lists]
+    int n_lists, list_len;
+};
+constexpr int kAppendThreads = 256;
+constexpr int kAppendDirect = 2048;
+constexpr int kAppendListLen = 4096;
+constexpr int kAppendMaxLists = 512;
+
+__device__ __forceinline__ int append_page_of(const CacheAppendArgs& a, int slot) {
+    const int page = slot >> a.page_shift;
+    return slot >= 0 && page < a.n_pages ? page : -1;
+}
+__device__ __forceinline__ bool append_run_begins(const CacheAppendArgs& a, int t, int page) {
+    return page >= 0 && (t == 0 || append_page_of(a, __ldg(a.slots + t - 1)) != page);
+}
+
+__global__ void __launch_bounds__(1024) smla_cache_runs_kernel(const CacheAppendArgs a) {
+    __shared__ int n;
+    if (threadIdx.x == 0) n = 0;
+    pdl_wait();
+    pdl_trigger();
+    __syncthreads();
+    const int t0 = blockIdx.x * a.list_len, t1 = min(t0 + a.list_len, a.n_rows);
+    for (int t = t0 + threadIdx.x; t < t1; t += 1024) {
+        const int page = append_page_of(a, __ldg(a.slots + t));
+        if (append_run_begins(a, t, page)) a.runs[t0 + atomicAdd(&n, 1)] = make_int2(page, t);     // (in any order)
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
+}
+
+struct AppendShared {
+    int win[kMaxPageRows];        // row of the call that goes to row r of the page, -1: none
+    int rows[kMaxPageRows];       // the page's rows that get one
+    int n_rows, earlier, end;
+    uint32_t warp_max[kAppendThreads / 32];
+};
+
+// The page's rows are known (win); quantise and write them.
+__device__ __forceinline__ void append_write_page(const CacheAppendArgs& a, int page, AppendShared& sh) {
+    constexpr int kUnits = kDQK / 8;              // 16 bytes of a bf16 row, 8 bytes of a stored one
+    const int page_rows = 1 << a.page_shift;
+    if (static_cast<int>(threadIdx.x) < page_rows && sh.win[threadIdx.x] >= 0) sh.rows[atomicAdd(&sh.n_rows, 1)] = threadIdx.x;
+    __syncthreads();
+    const int n_units = sh.n_rows * kUnits;
+    auto source = [&](int u) {
+        const int i = u / kUnits;
+        return reinterpret_cast<const uint4*>(a.kv + static_cast<long long>(sh.win[sh.rows[i]]) * a.kv_stride) + (u - i * kUnits);
+    };
+    uint32_t top = 0;                             // largest finite |x|, as the bits of an fp32 number
+#pragma unroll 4
+    for (int u = threadIdx.x; u < n_units; u += kAppendThreads) {
+        const uint4 v = __ldg(source(u));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = (w[k] << 16) & 0x7fff0000u, hi = w[k] & 0x7fff0000u;
+            top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) sh.warp_max[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, sh.warp_max[w]);
+    const float wanted = exp2_int(scale_exp(top));
+    const float old = a.scales[page];
+    const bool anew = sh.win[0] >= 0;             // its first row is written: what it held belongs to nobody
+    const float scale = anew ? wanted : fmaxf(old, wanted);
+    __syncthreads();                              // (the old scale has been read)
+    uint8_t* base = a.values + static_cast<size_t>(page) * page_rows * kDQK;
+    if (!anew && scale > old) {
+        const float ratio = old / scale;
+        for (int u = threadIdx.x; u < page_rows * (kDQK / 16); u += kAppendThreads) {
+            const int r = u / (kDQK / 16);
+            if (sh.win[r] >= 0) continue;
+            uint4* at = reinterpret_cast<uint4*>(base + static_cast<size_t>(u) * 16);
+            const uint4 v = *at;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 lo = e4m3x2_to_float2(w[k] & 0xffffu), hi = e4m3x2_to_float2(w[k] >> 16);
+                w[k] = cvt_e4m3x2(lo.x * ratio, lo.y * ratio) | cvt_e4m3x2(hi.x * ratio, hi.y * ratio) << 16;
+            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    if (threadIdx.x == 0) a.scales[page] = scale;
+    const float inv = 1.f / scale;
+    // an infinity is stored as a NaN: the format has none, and it has no place among finite numbers
+    auto scaled = [&](uint32_t bits) { return (bits & 0x7fffffffu) < 0x7f800000u ? __uint_as_float(bits) * inv : __uint_as_float(0x7fffffffu); };
+#pragma unroll 4
+    for (int u = threadIdx.x; u < n_units; u += kAppendThreads) {
+        const uint4 v = __ldg(source(u));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t c[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c[k] = cvt_e4m3x2(scaled(w[k] << 16), scaled(w[k] & 0xffff0000u));
+        const int i = u / kUnits;
+        *reinterpret_cast<uint2*>(base + static_cast<size_t>(sh.rows[i]) * kDQK + (u - i * kUnits) * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    }
+}
+
+__device__ __forceinline__ void append_clear(AppendShared& sh) {
+    if (threadIdx.x < kMaxPageRows) sh.win[threadIdx.x] = -1;
+    if (threadIdx.x == 0) sh.n_rows = sh.earlier = 0;
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(kAppendThreads) smla_cache_append_kernel(const CacheAppendArgs a) {
+    __shared__ AppendShared sh;
+    const int row_mask = (1 << a.page_shift) - 1;
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.x, page = append_page_of(a, __ldg(a.slots + t));
+    if (!append_run_begins(a, t, page)) return;
+    append_clear(sh);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < a.n_rows; i += kAppendThreads) {
+        const int slot = __ldg(a.slots + i);
+        if (append_page_of(a, slot) == page) {
+            if (i < t) sh.earlier = 1;
+            atomicMax(&sh.win[slot & row_mask], i);
+        }
+    }
+    __syncthreads();
+    if (sh.earlier) return;                       // the page's first run does it
+    append_write_page(a, page, sh);
+}
+
+__global__ void __launch_bounds__(kAppendThreads) smla_cache_append_listed_kernel(const CacheAppendArgs a) {
+    __shared__ AppendShared sh;
+    __shared__ int before[kAppendMaxLists + 1];   // runs in the lists before
+    const int row_mask = (1 << a.page_shift) - 1;
+    pdl_wait();
+    pdl_trigger();
+    if (threadIdx.x < 32) {
+        int carry = 0;
+        for (int l0 = 0; l0 < a.n_lists; l0 += 32) {
+            const int l = l0 + threadIdx.x, c = l < a.n_lists ? __ldcg(a.counts + l) : 0;
+            int incl = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (static_cast<int>(threadIdx.x) >= o) incl += up;
+            }
+            if (l < a.n_lists) before[l] = carry + incl - c;
+            carry += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (threadIdx.x == 0) before[a.n_lists] = carry;
+    }
+    __syncthreads();
+    const int n_runs = before[a.n_lists];
+    auto run = [&](int g) {
+        const int l = last_not_above(before, a.n_lists, g);
+        return __ldcg(a.runs + static_cast<size_t>(l) * a.list_len + (g - before[l]));
+    };
+    for (int item = blockIdx.x; item < n_runs; item += gridDim.x) {
+        const int2 mine = run(item);
+        append_clear(sh);
+        auto take = [&](int t) { atomicMax(&sh.win[__ldg(a.slots + t) & row_mask], t); };
+        auto in_run = [&](int t) { return t < a.n_rows && append_page_of(a, __ldg(a.slots + t)) == mine.x; };
+        for (int g = threadIdx.x; g < n_runs; g += kAppendThreads) {
+            const int2 other = run(g);
+            if (other.x != mine.x || other.y == mine.y) continue;
+            if (other.y < mine.y) sh.earlier = 1;
+            else
+                for (int t = other.y; in_run(t); ++t) take(t);         // (seldom: the page comes up again)
+        }
+        __syncthreads();
+        if (!sh.earlier) {
+            for (int t0 = mine.y;; t0 += kAppendThreads) {
+                if (threadIdx.x == 0) sh.end = a.n_rows;
+                __syncthreads();
+                const int t = t0 + threadIdx.x;
+                if (!in_run(t)) atomicMin(&sh.end, t);
+                __syncthreads();
+                const int end = sh.end;
+                if (t < end) take(t);
+                __syncthreads();
+                if (end < t0 + kAppendThreads) break;
+            }
+            append_write_page(a, mine.x, sh);
+        }
+        __syncthreads();                          // (the next page's tables go to the same place)
+    }
+}
+
+}  // namespace smla

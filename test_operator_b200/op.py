@@ -19,7 +19,7 @@ import math
 import os
 import threading
 import warnings
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -51,6 +51,23 @@ class _FwdParams(ctypes.Structure):
         ("sm_scale", ctypes.c_float), ("q_start_index_s", ctypes.c_int32), ("lse_is_base2", ctypes.c_int32),
         ("query_meta", ctypes.c_void_p),
     ]
+
+
+class _CachePlanParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("kv_len", "new_len", "free_count", "block_table", "free_pages", "slots", "query_meta", "kv_len_out",
+                                               "free_count_out", "admitted")] + \
+               [(n, ctypes.c_int32) for n in ("n_requests", "max_pages", "n_free", "page_size", "max_tokens", "topk")]
+
+
+class _CacheAppendParams(ctypes.Structure):
+    _fields_ = [("kv", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("values", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("kv_stride", ctypes.c_int64), ("n_rows", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+
+class _FwdCachedParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "values", "scales", "block_table", "indices", "query_meta", "o", "lse")] + \
+               [(n, ctypes.c_int32) for n in ("s_q", "h_q", "topk", "n_pages", "page_size", "n_requests", "max_pages")] + \
+               [("sm_scale", ctypes.c_float), ("causal", ctypes.c_int32), ("lse_is_base2", ctypes.c_int32)]
 
 
 class _DetParams(ctypes.Structure):
@@ -130,6 +147,16 @@ def load_library() -> ctypes.CDLL:
         lib.smla_fwd_workspace_size.argtypes = [ctypes.POINTER(_FwdParams), ctypes.c_size_t]
         lib.smla_fwd_run.restype = ctypes.c_int
         lib.smla_fwd_run.argtypes = [ctypes.POINTER(_FwdParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.smla_cache_plan.restype = ctypes.c_int
+        lib.smla_cache_plan.argtypes = [ctypes.POINTER(_CachePlanParams), ctypes.c_void_p]
+        lib.smla_cache_append_workspace_size.restype = ctypes.c_size_t
+        lib.smla_cache_append_workspace_size.argtypes = [ctypes.c_int32]
+        lib.smla_cache_append.restype = ctypes.c_int
+        lib.smla_cache_append.argtypes = [ctypes.POINTER(_CacheAppendParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.smla_fwd_cached_workspace_size.restype = ctypes.c_size_t
+        lib.smla_fwd_cached_workspace_size.argtypes = [ctypes.POINTER(_FwdCachedParams), ctypes.c_size_t]
+        lib.smla_fwd_cached_run.restype = ctypes.c_int
+        lib.smla_fwd_cached_run.argtypes = [ctypes.POINTER(_FwdCachedParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.smla_bwd_last_launch_count.restype = ctypes.c_int
         lib.smla_index_inverse_workspace_size.restype = ctypes.c_size_t
         lib.smla_index_inverse_workspace_size.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
@@ -678,6 +705,182 @@ class SparseMLAFunction(torch.autograd.Function):
 def sparse_mla(q, kv, indices, sm_scale: Optional[float] = None, q_start_index_s: Optional[int] = 0):
     """Differentiable sparse MLA attention (bf16 in, bf16 out; gradients for q and kv)."""
     return SparseMLAFunction.apply(q, kv, indices, sm_scale, q_start_index_s)
+
+
+# ---- serving: a paged cache of kv rows in 8 bits --------------------------------------------------------------------------------
+_PAGE_SIZES = (16, 32, 64, 128)
+
+
+class LatentCache(NamedTuple):
+    """A paged cache of kv rows in 8 bits: `values` float8_e4m3fn [n_pages, page_size, 576] and `scales` fp32 [n_pages], one power of two for
+    all rows of a page; a stored number times its page's scale is the kv value.  page_size: 16, 32, 64 or 128.  A row's slot is
+    page * page_size + row.  Any two such tensors will do; `empty` allocates a pair."""
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, device) -> "LatentCache":
+        _check(page_size in _PAGE_SIZES, f"page_size must be one of {_PAGE_SIZES}, got {page_size}")
+        return cls(torch.zeros(n_pages, page_size, D_QK, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                   torch.zeros(n_pages, dtype=torch.float32, device=device))
+
+    @property
+    def page_size(self) -> int:
+        return self.values.shape[1]
+
+
+class CachePlan(NamedTuple):
+    """What `cache_plan` makes of a step (int32, on the device)."""
+    slots: torch.Tensor         # [max_tokens] slot of each new token, -1: none
+    query_meta: torch.Tensor    # [max_tokens, 4] what `mla_fwd_cached` takes
+    kv_len: torch.Tensor        # [n_requests] tokens in the cache after the step
+    free_count: torch.Tensor    # [1] free pages after the step
+    admitted: torch.Tensor      # [n_requests] new tokens that have a slot
+
+
+def _check_int32(t, shape, device, name) -> None:
+    _check(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 CUDA tensor")
+    _check(t.device == device, f"{name} must be on {device}")
+    _check(t.dim() == len(shape) and all(want is None or have == want for have, want in zip(t.shape, shape)),
+           f"{name} must have shape {[('*' if n is None else n) for n in shape]}, got {list(t.shape)}")
+
+
+def _check_cache(cache, device) -> None:
+    _check(isinstance(cache, tuple) and len(cache) == 2 and all(isinstance(t, torch.Tensor) for t in cache), "cache must be a LatentCache")
+    values, scales = cache
+    _check(values.is_cuda and scales.is_cuda and values.device == device and scales.device == device, f"the cache must be on {device}")
+    _check(values.dtype == torch.float8_e4m3fn and scales.dtype == torch.float32, "a cache holds float8_e4m3fn values and float32 scales")
+    _check(values.dim() == 3 and values.shape[0] > 0 and values.shape[1] in _PAGE_SIZES and values.shape[2] == D_QK and values.is_contiguous(),
+           f"cache values must be contiguous [n_pages, page_size, {D_QK}] with a page_size of {_PAGE_SIZES}")
+    _check(scales.dim() == 1 and scales.shape[0] == values.shape[0] and scales.is_contiguous(), "cache scales must be contiguous [n_pages]")
+    _check(values.shape[0] * values.shape[1] < 2 ** 31, "a cache holds less than 2^31 rows")
+
+
+def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+               page_size: int, max_tokens: int, topk: int) -> CachePlan:
+    """Tables of one serving step, made on the GPU from the requests' lengths: pages for the new tokens, the slot of each of them, and the
+    query table of `mla_fwd_cached`.  All tensors int32 on one device.
+
+    kv_len [n_requests]: tokens each request has in the cache; new_len [n_requests]: how many it gets in this step, or a negative number
+    for a request that ends and gives its pages back.  block_table [n_requests, max_pages] and free_pages (a stack whose first
+    free_count[0] entries are free pages) are updated in place; kv_len, new_len and free_count are not changed: the plan holds their
+    successors.  Token rows are packed in order of requests, new_len[i] of each; rows behind the last of them, up to max_tokens (a fixed
+    size for a step that is captured in a graph), have slot -1 and an empty query.  Requests are served in order; one for which the pages, the
+    table's width or the rows do not suffice gets nothing in this step (`admitted` 0, its rows' slots -1), nor does a later one that needs a
+    page once there were too few.  At most 8192 requests; nothing synchronises."""
+    _check(isinstance(kv_len, torch.Tensor) and kv_len.is_cuda, "kv_len must be a CUDA tensor")
+    device = kv_len.device
+    _check_int32(kv_len, (None,), device, "kv_len")
+    n = kv_len.shape[0]
+    _check(0 < n <= 8192, f"cache_plan takes 1 to 8192 requests, got {n}")
+    _check_int32(new_len, (n,), device, "new_len")
+    _check_int32(block_table, (n, None), device, "block_table")
+    _check_int32(free_pages, (None,), device, "free_pages")
+    _check_int32(free_count, (1,), device, "free_count")
+    _check(page_size in _PAGE_SIZES, f"page_size must be one of {_PAGE_SIZES}, got {page_size}")
+    _check(0 <= max_tokens < 2 ** 30 and 0 <= topk < 2 ** 31, "max_tokens must be in [0, 2^30), topk in [0, 2^31)")
+    _check(block_table.shape[1] > 0 and free_pages.shape[0] > 0, "block_table and free_pages must not be empty")
+    _check(block_table.shape[1] * page_size <= 2 ** 30 and block_table.numel() + free_pages.numel() < 2 ** 31,
+           "a request holds at most 2^30 tokens, block_table and free_pages less than 2^31 entries together")
+    lib = load_library()
+    index = kv_len.get_device()
+    with _on_device(index):
+        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=device)  # noqa: E731
+        plan = CachePlan(new(max_tokens), new(max_tokens, 4), new(n), new(1), new(n))
+        p = _CachePlanParams(kv_len.data_ptr(), new_len.data_ptr(), free_count.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
+                             plan.slots.data_ptr(), plan.query_meta.data_ptr(), plan.kv_len.data_ptr(), plan.free_count.data_ptr(),
+                             plan.admitted.data_ptr(), n, block_table.shape[1], free_pages.shape[0], page_size, max_tokens, topk)
+        _raise_status(lib, lib.smla_cache_plan(ctypes.byref(p), _raw_stream(index)), "smla_cache_plan")
+    return plan
+
+
+def cache_append(kv: torch.Tensor, cache: LatentCache, slots: torch.Tensor) -> None:
+    """Write kv rows (bf16 [n, 576], or [n, 1, 576]; rows may be strided by a multiple of 8 elements) into `cache` at `slots` (int32 [n], -1: leave out).
+
+    Rows are rounded to e4m3 against their page's scale.  A page whose row 0 is among the slots starts anew: its scale becomes the
+    smallest power of two (2^-100 at least) that holds the rows it gets now.  Any other page's scale grows where they need it, and the rows
+    it keeps are brought over.  Of several rows with one slot the last one is kept; slots may come in any order, and ones outside the cache
+    are left out.  A number that is not finite is stored as a NaN.  Enqueues on the current stream; calls on one cache must be ordered."""
+    _check(isinstance(kv, torch.Tensor) and kv.is_cuda and kv.dtype == torch.bfloat16, "kv must be a bfloat16 CUDA tensor")
+    if kv.dim() == 3 and kv.shape[1] == 1:
+        kv = kv[:, 0]
+    _check(kv.dim() == 2 and kv.shape[1] == D_QK, f"kv must have shape [n, {D_QK}] or [n, 1, {D_QK}]")
+    n = kv.shape[0]
+    _check(kv.stride(1) == 1 and (n <= 1 or kv.stride(0) % 8 == 0) and kv.data_ptr() % 16 == 0,
+           "kv rows must be contiguous, 16-byte aligned, and a multiple of 8 elements apart")
+    _check_cache(cache, kv.device)
+    _check_int32(slots, (n,), kv.device, "slots")
+    if n == 0:
+        return
+    lib = load_library()
+    index = kv.get_device()
+    with _on_device(index):
+        need = lib.smla_cache_append_workspace_size(n)
+        ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+        p = _CacheAppendParams(kv.data_ptr(), slots.data_ptr(), cache.values.data_ptr(), cache.scales.data_ptr(), kv.stride(0) if n > 1 else D_QK, n,
+                               cache.values.shape[0], cache.values.shape[1])
+        st = lib.smla_cache_append(ctypes.byref(p), ws.data_ptr() if need else None, need, _raw_stream(index))
+    _raise_status(lib, st, "smla_cache_append")
+
+
+@functools.lru_cache(maxsize=4096)
+def _fwd_cached_workspace_bytes(s_q: int, h_q: int, topk: int, n_pages: int, page_size: int, n_requests: int, max_pages: int, budget: int) -> int:
+    p = _FwdCachedParams(0, 0, 0, 0, 0, 0, 0, 0, s_q, h_q, topk, n_pages, page_size, n_requests, max_pages, 0.0, 1, 1)
+    return load_library().smla_fwd_cached_workspace_size(ctypes.byref(p), budget)
+
+
+def mla_fwd_cached(q: torch.Tensor, cache: LatentCache, block_table: torch.Tensor, indices: torch.Tensor, query_meta: torch.Tensor,
+                   sm_scale: Optional[float] = None, causal: bool = True, lse_is_base2: bool = True, workspace: Optional[Workspace] = None,
+                   workspace_budget: int = 0, check_device_status: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`mla_fwd` over a paged 8-bit cache: returns (o bf16 [s_q, h_q, 512], lse fp32 [s_q, h_q]).
+
+    `block_table` [n_requests, max_pages] names the pages of each request; `indices` [s_q, topk] (or [s_q, 1, topk]) are positions in the
+    query's own request; `query_meta` [s_q, 4] is what `cache_plan` makes: request, its tokens in the cache, the query's position, top-k slots
+    in use (all int32).  A slot counts if it is in use, its position lies in the request's tokens and, with `causal`, not behind the query's,
+    and its page is one of the cache.  A query without such a slot (a padding row) gives o = 0 and lse = +inf.  Of a page's scale the exponent
+    is used.  Prompts and single tokens take the same call."""
+    for name, t in (("q", q), ("indices", indices)):
+        _check(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous(), f"{name} must be a contiguous CUDA tensor")
+    _check(q.dtype == torch.bfloat16 and indices.dtype == torch.int32, "dtypes: q bfloat16, indices int32")
+    _check(q.dim() == 3 and q.shape[2] == D_QK, f"q must have shape [s_q, h_q, {D_QK}]")
+    s_q, h_q, _ = q.shape
+    _check(0 < h_q <= 128 and h_q % 8 == 0, f"h_q must be a multiple of 8 in [8, 128], got {h_q}")
+    _check(indices.shape[0] == s_q and (indices.dim() == 2 or (indices.dim() == 3 and indices.shape[1] == 1)), "indices must be [s_q,topk] or [s_q,1,topk]")
+    _check(indices.device == q.device, "indices must be on the same device as q")
+    topk = indices.shape[-1]
+    _check(topk > 0, "topk must be positive")
+    _check_cache(cache, q.device)
+    _check_int32(block_table, (None, None), q.device, "block_table")
+    _check_int32(query_meta, (s_q, 4), q.device, "query_meta")
+    _check(query_meta.data_ptr() % 16 == 0, "query_meta must be 16-byte aligned")
+    n_pages, page_size = cache.values.shape[:2]
+    n_req, max_pages = block_table.shape
+    _check(n_req > 0 and 0 < max_pages * page_size <= 2 ** 30, "block_table must not be empty, and a request holds at most 2^30 tokens")
+    lib = load_library()
+    index = q.get_device()
+    with _on_device(index):
+        o = torch.empty((s_q, h_q, D_V), dtype=torch.bfloat16, device=q.device)
+        lse = torch.empty((s_q, h_q), dtype=torch.float32, device=q.device)
+        if s_q == 0:
+            return o, lse
+        p = _FwdCachedParams(q.data_ptr(), cache.values.data_ptr(), cache.scales.data_ptr(), block_table.data_ptr(), indices.data_ptr(),
+                             query_meta.data_ptr(), o.data_ptr(), lse.data_ptr(), s_q, h_q, topk, n_pages, page_size, n_req, max_pages,
+                             float(sm_scale) if sm_scale is not None else 0.0, 1 if causal else 0, 1 if lse_is_base2 else 0)
+        if workspace is None:
+            # allocated per call, as in mla_fwd
+            need = _fwd_cached_workspace_bytes(s_q, h_q, topk, n_pages, page_size, n_req, max_pages, workspace_budget)
+            _check(need > 0, "unsupported shapes for the forward over a cache")
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+            if check_device_status:
+                scratch[:256].zero_()
+            ptr = scratch.data_ptr()
+        else:
+            ptr, need = workspace.ptr, workspace.nbytes
+        stream = _raw_stream(index)
+        _raise_status(lib, lib.smla_fwd_cached_run(ctypes.byref(p), ptr, need, stream), "smla_fwd_cached_run")
+        if check_device_status:
+            _raise_status(lib, lib.smla_bwd_status(ptr, stream), "smla_fwd_cached device status")
+    return o, lse
 
 
 def index_inverse(indices: torch.Tensor, s_kv: int, q_start_index_s: Optional[int] = None):
