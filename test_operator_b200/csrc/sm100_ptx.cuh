@@ -98,15 +98,18 @@ __device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, const W
     if (mbar_test_wait(bar, parity)) return true;
     return mbar_spin_slow(bar, parity, ctx, code);
 }
+__device__ __forceinline__ void mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int code, unsigned sleep_ns = 0);
 // The consumer's place in a ring of slots, with the barrier of the NEXT slot polled while the current one is worked on, so
 // that a poll's latency is not added to every slot of a thread that issues UMMAs (or forwards signals) one slot at a time.
-template <int kSlots> struct RingReader {
+template <int kSlots, bool kSpin = true> struct RingReader {
     uint32_t full0;               // barrier of slot 0
     uint32_t slot = 0, phase = 0;
     bool ready = false;           // the current slot has been seen full
     __device__ __forceinline__ explicit RingReader(uint32_t full0_) : full0(full0_) {}
     __device__ __forceinline__ void wait(const WaitCtx& ctx, int code) {
-        if (!ready) mbar_spin(full0 + 8 * slot, phase, ctx, code);
+        if (ready) return;
+        if constexpr (kSpin) mbar_spin(full0 + 8 * slot, phase, ctx, code);
+        else mbar_wait_inline(full0 + 8 * slot, phase, ctx, code);
     }
     // to the next slot, polling it; call before the work on `slot`'s data is issued, with the old slot number kept
     __device__ __forceinline__ void next() {
@@ -139,6 +142,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
                                           unsigned sleep_ns = 0) {
     if (mbar_try_wait(bar, parity)) return true;
     return mbar_wait_slow(bar, parity, ctx, code, sleep_ns);
+}
+
+// The same without a call on its slow path, for kernels that have no register to spare: what lives across a call is spilled.
+__device__ __forceinline__ void mbar_wait_inline(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int code, unsigned sleep_ns) {
+    if (mbar_try_wait(bar, parity)) return;
+    const long long t0 = clock64();
+    for (int it = 1; !mbar_try_wait(bar, parity); ++it) {
+        if (sleep_ns) __nanosleep(sleep_ns);
+        if ((it & 31) == 0) {
+            if (*ctx.s_abort) return;
+            if (clock64() - t0 > ctx.limit) {
+                wait_give_up(ctx, code);
+                return;
+            }
+        }
+    }
 }
 
 // Wait used only while a CTA winds down after an abort: ignores the abort flag, still bounded.
@@ -181,6 +200,8 @@ __device__ __forceinline__ bool flag_wait(uint32_t saddr, uint32_t want, const W
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
+// (global memory too)
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before_sync() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -208,6 +229,8 @@ __device__ __forceinline__ uint64_t l2_policy_evict_first() {
     return pol;
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // ---- TMA ---------------------------------------------------------------------------------------
 // Tiled loads: box as encoded in the tensor map, coordinates {c0 = innermost element, c1 = row, ...}.
 // c0 * element size must be a multiple of 16 bytes.
@@ -227,6 +250,11 @@ __device__ __forceinline__ void tma_load_4d_hint(uint32_t dst, const void* tmap,
         ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
         : "memory");
 }
+// Bulk copy of `bytes` (multiple of 16, both addresses 16-byte aligned) from global to this CTA's shared memory, counted on its barrier `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t sdst, const void* gsrc, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sdst), "l"(gsrc), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 // Bulk copy of `bytes` (multiple of 16, both addresses 16-byte aligned) from this CTA's shared memory to global,
 // tracked by the thread's bulk-group; the source may be reused after bulk_wait_read().
 __device__ __forceinline__ void bulk_store(void* gdst, uint32_t ssrc, uint32_t bytes) {
@@ -244,6 +272,24 @@ __device__ __forceinline__ void st_shared_v4(uint32_t saddr, uint32_t a, uint32_
 }
 __device__ __forceinline__ void st_shared_v2(uint32_t saddr, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(saddr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t saddr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(saddr), "f"(v) : "memory"); }
+__device__ __forceinline__ float ld_shared_f32(uint32_t saddr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(saddr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_s32(uint32_t saddr, int v) { asm volatile("st.shared.s32 [%0], %1;" ::"r"(saddr), "r"(v) : "memory"); }
+__device__ __forceinline__ int4 ld_shared_s32x4(uint32_t saddr) {
+    int4 v;
+    asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(saddr) : "memory");
+    return v;
+}
+// four fp32 as two packed pairs
+__device__ __forceinline__ ulonglong2 ld_shared_f32x4(uint32_t saddr) {
+    ulonglong2 v;
+    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(saddr) : "memory");
+    return v;
 }
 // Copies `src_bytes` (0 or 16) bytes and fills the rest of the 16 with zeros: with 0 nothing is read from global.
 __device__ __forceinline__ void cp_async16_zfill_hint(uint32_t dst, const void* src, uint32_t src_bytes, uint64_t policy) {
@@ -486,6 +532,37 @@ __device__ __forceinline__ float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two fp32 numbers in one 64-bit register and the packed arithmetic on them.
+__device__ __forceinline__ uint64_t pack_f32x2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float max3_f32(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 // two fp32 -> packed bf16x2 (round to nearest even); `lo` goes to the low half
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
