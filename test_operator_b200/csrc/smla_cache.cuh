@@ -37,6 +37,17 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float 
         : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
+// Four numbers as the sum of two e4m3 numbers each: the nearest one (hi), and the one that is nearest to what it leaves (lo).
+__device__ __forceinline__ void split_e4m3x4(uint64_t x01, uint64_t x23, uint32_t* hi, uint32_t* lo) {
+    const float2 a = unpack_f32x2(x01), b = unpack_f32x2(x23);
+    *hi = cvt_e4m3x4(a.x, a.y, b.x, b.y);
+    uint32_t h01, h23;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(h01), "=r"(h23) : "r"(*hi));
+    const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h01)), d = __half22float2(*reinterpret_cast<const __half2*>(&h23));
+    const uint64_t minus = pack_f32x2(-1.f, -1.f);
+    const float2 e = unpack_f32x2(fma_f32x2(pack_f32x2(c.x, c.y), minus, x01)), f = unpack_f32x2(fma_f32x2(pack_f32x2(d.x, d.y), minus, x23));
+    *lo = cvt_e4m3x4(e.x, e.y, f.x, f.y);
+}
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));

@@ -4,9 +4,9 @@
 // what differs.
 //   operands   kind::f8f6f4 UMMAs on the stored e4m3 numbers as they lie, for K and for V: nothing is converted on the way, and a
 //              gathered row is 576 bytes instead of 1152.  The other side of either product is the sum of two e4m3 numbers, one UMMA each:
-//              q = 2^e (hi + lo) with e from the row's largest magnitude.  A bf16 number has eight significant bits; hi takes four, lo the
-//              other four, so hi + lo is q exactly for what is within 2^-10 of the row's largest, and within 2^-19 of the largest for the rest.
-//              P hi + lo likewise: eight significant bits, what bf16 has, and steps of 2^-9 below 2^-2.
+//              q = 2^e (hi + lo) with e from the row's largest magnitude.  A bf16 number has eight significant bits; hi takes four,
+//              what it leaves has four at most, so hi + lo is q exactly for what is within 2^-10 of the row's largest, and within half of
+//              2^-9, 2^-17.8 of the largest, for the rest.  P hi + lo likewise: within 2^-9 of P, bf16's is 2^-8, and within half of 2^-9.
 //              An 8-bit UMMA takes 32 of K in the time of 16 in bf16, so two of them cost what one contraction in bf16 costs.
 //   scales     of a key's page, s_j.  The logits are x_j = scale 2^e s_j (hi + lo) c_j.  V needs p_j s_j, and that is what is rounded:
 //              P_j = 2^(x_j + log2 s_j - ref), so that the heaviest P_j are alike whatever the pages' scales are: with ref set the
@@ -91,28 +91,22 @@ __device__ __noinline__ void split_row(const __nv_bfloat16* row, uint32_t image,
     const int e = bad ? 0 : scale_exp(top);
     const float f = bad ? __int_as_float(0x7fffffff) : exp2_int(-e);
     if (u == 0) st_shared_f32(exps + r * 4, exp2_int(e));
-    const uint64_t f2 = pack_f32x2(f, f), minus = pack_f32x2(-1.f, -1.f);
+    const uint64_t f2 = pack_f32x2(f, f);
     const uint32_t to = image + r * 128 + (u & 1) * 8;
 #pragma unroll
     for (int j = 0; j < 9; ++j) {
         const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-        float h[8], l[8];
+        uint64_t x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint64_t x2 = mul_f32x2(pack_f32x2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)), f2);
-            const float2 x = unpack_f32x2(x2);
-            // four significant bits, and what they leave
-            h[2 * k] = __uint_as_float(__float_as_uint(x.x) & 0xfff00000u);
-            h[2 * k + 1] = __uint_as_float(__float_as_uint(x.y) & 0xfff00000u);
-            const float2 left = unpack_f32x2(fma_f32x2(pack_f32x2(h[2 * k], h[2 * k + 1]), minus, x2));
-            l[2 * k] = left.x;
-            l[2 * k + 1] = left.y;
-        }
+        for (int k = 0; k < 4; ++k) x[k] = mul_f32x2(pack_f32x2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)), f2);
+        uint32_t h[2], l[2];
+        split_e4m3x4(x[0], x[1], &h[0], &l[0]);
+        split_e4m3x4(x[2], x[3], &h[1], &l[1]);
         const int unit = (j & 1) * 4 + (u >> 1);
         const uint32_t to_hi = to + (j >> 1) * 2 * kTerm + ((unit ^ (r & 7)) << 4);
         const uint32_t to_lo = j < 8 ? to_hi + kTerm : to + 8 * kTerm + (((4 + unit) ^ (r & 7)) << 4);
-        st_shared_v2(to_hi, cvt_e4m3x4(h[0], h[1], h[2], h[3]), cvt_e4m3x4(h[4], h[5], h[6], h[7]));
-        st_shared_v2(to_lo, cvt_e4m3x4(l[0], l[1], l[2], l[3]), cvt_e4m3x4(l[4], l[5], l[6], l[7]));
+        st_shared_v2(to_hi, h[0], h[1]);
+        st_shared_v2(to_lo, l[0], l[1]);
     }
 }
 
@@ -575,29 +569,20 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
             }
             const float neg = ref == ninf ? 0.f : -ref;
             sum *= scale_o;
-            const uint64_t neg2 = pack_f32x2(neg, neg), minus = pack_f32x2(-1.f, -1.f);
+            const uint64_t neg2 = pack_f32x2(neg, neg);
             uint64_t add = 0;
             uint32_t p_hi[8], p_lo[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const ulonglong2 inv = ld_shared_f32x4(scale_s + 2 * kTileKeys * 4 + 16 * i);
-                float x[4], h[4], l[4];
+                uint64_t x[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const float2 z = unpack_f32x2(add_f32x2(y[2 * i + k], neg2));
-                    x[2 * k] = ex2_approx(z.x);
-                    x[2 * k + 1] = ex2_approx(z.y);
-                    const uint64_t x2 = pack_f32x2(x[2 * k], x[2 * k + 1]);
-                    add = fma_f32x2(x2, k ? inv.y : inv.x, add);
-                    // four significant bits, and what they leave
-                    h[2 * k] = __uint_as_float(__float_as_uint(x[2 * k]) & 0xfff00000u);
-                    h[2 * k + 1] = __uint_as_float(__float_as_uint(x[2 * k + 1]) & 0xfff00000u);
-                    const float2 left = unpack_f32x2(fma_f32x2(pack_f32x2(h[2 * k], h[2 * k + 1]), minus, x2));
-                    l[2 * k] = left.x;
-                    l[2 * k + 1] = left.y;
+                    x[k] = pack_f32x2(ex2_approx(z.x), ex2_approx(z.y));
+                    add = fma_f32x2(x[k], k ? inv.y : inv.x, add);
                 }
-                p_hi[i] = cvt_e4m3x4(h[0], h[1], h[2], h[3]);
-                p_lo[i] = cvt_e4m3x4(l[0], l[1], l[2], l[3]);
+                split_e4m3x4(x[0], x[1], &p_hi[i], &p_lo[i]);
             }
             {
                 const float2 v = unpack_f32x2(add);

@@ -36,3 +36,11 @@ def queries(kv_len, new, topk, rng, pad=0, unused=0.1):
 
 def on(device, *arrays):
     return [torch.from_numpy(np.ascontiguousarray(a)).to(device) for a in arrays]
+
+
+def share_of_bound(got, want, bound):
+    """The largest difference as a share of what it may be; above 1 where only one of the two is a NaN."""
+    if not got.numel():
+        return 0.0
+    share = torch.where((got.double() == want) | (got.isnan() & want.isnan()), 0.0, (got.double() - want).abs() / bound)
+    return float(share.nan_to_num(nan=1e9, posinf=1e9).max())

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle.latent_cache_ref import attend_ref
-from tests.cache_inputs import on, queries, random_cache, requests
+from tests.cache_inputs import on, queries, random_cache, requests, share_of_bound
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -35,20 +35,12 @@ def _run(q, values, scales, table, idx, meta, **kwargs):
     return op.mla_fwd_cached(q, op.LatentCache(values, scales), table, idx, meta, check_device_status=True, **kwargs)
 
 
-def _share(got, want, bound):
-    """The largest difference as a share of what it may be; above 1 where only one of the two is a NaN."""
-    if not got.numel():
-        return 0.0
-    share = torch.where((got.double() == want) | (got.isnan() & want.isnan()), 0.0, (got.double() - want).abs() / bound)
-    return float(share.nan_to_num(nan=1e9, posinf=1e9).max())
-
-
 def _compare(o, lse, ref):
     none = ref.lse.isposinf()
     assert int((lse.isposinf() != none).sum()) == 0 and int(o[none].count_nonzero()) == 0
-    assert _share(o, ref.o, ref.o_bound) <= 1
+    assert share_of_bound(o, ref.o, ref.o_bound) <= 1
     fine = ~none
-    assert _share(lse[fine], ref.lse[fine], ref.lse_bound[fine]) <= 1
+    assert share_of_bound(lse[fine], ref.lse[fine], ref.lse_bound[fine]) <= 1
     # roundings are of either sign: together they come to less than one of them (half a step of bf16 and of P, each at most 2^-8 and 2^-9 on average)
     off = (o.double() - ref.o)[~ref.o.isnan()]
     assert off.norm() <= 2 ** -8 * ref.o[~ref.o.isnan()].norm()
@@ -182,7 +174,7 @@ def test_what_is_not_a_number_stays_none(kind, s_q):
     o, lse = _run(q, values, scales, table, idx, meta)
     assert torch.equal(o.isnan().any(2), hit) and torch.equal(o.isnan().all(2), hit if kind != "kv_nan" else o.isnan().all(2)) and torch.equal(lse.isnan(), hit)
     fine = ~hit
-    assert _share(o[fine], ref.o[fine], ref.o_bound[fine]) <= 1
+    assert share_of_bound(o[fine], ref.o[fine], ref.o_bound[fine]) <= 1
 
 
 def test_same_bits_every_time_and_on_every_stream():
