@@ -1,10 +1,12 @@
-// Host side of the two operator calls as a small CPython module: one look at the tensors, the outputs' allocation and the C ABI
+// Host side of the operator calls as a small CPython module: one look at the tensors, the outputs' allocation and the C ABI
 // call (include/smla_bwd.h) without a trip through the interpreter for each.  It holds no kernels: the library that op.py has
 // loaded hands its entry points over (init).
 //
 // Why: the smallest calls keep the GPU busy for 15 - 20 us, and a call's way through Python took the host as long.  Host time of a
 // call, through Python / so: backward of 64 queries x 16 heads x top-k 64 (three launches) 23.7 / 12.4 us, forward of eight tokens x 128
-// heads (two) 17.0 / 8.0; from an idle GPU to the result 46.1 / 34.9 and 42.0 / 33.3.
+// heads (two) 17.0 / 8.0; from an idle GPU to the result 46.1 / 34.9 and 42.0 / 33.3.  The calls of a serving step (tables, rows into the
+// cache, forward over it), whose kernels take 2 - 17 us: tables of
+// 8 requests 32.5 / 6.4 us a call, 8 rows into the cache 13.4 / 3.7, one token x 128 heads over it 29.5 / 16.8 (its kernels' time).
 //
 // It takes what nearly every call passes and answers None (or a size of 0) for anything else - other argument types, tensor
 // subclasses, wrapped tensors, wrong shapes - which op.py then handles itself, error messages included.
@@ -35,6 +37,11 @@ decltype(&smla_fwd_run) g_fwd_run = nullptr;
 decltype(&smla_fwd_workspace_size) g_fwd_size = nullptr;
 decltype(&smla_bwd_run_stages) g_bwd_run = nullptr;
 decltype(&smla_bwd_workspace_size) g_bwd_size = nullptr;
+decltype(&smla_cache_plan) g_cache_plan = nullptr;
+decltype(&smla_cache_append) g_cache_append = nullptr;
+decltype(&smla_cache_append_workspace_size) g_append_size = nullptr;
+decltype(&smla_fwd_cached_run) g_cached_run = nullptr;
+decltype(&smla_fwd_cached_workspace_size) g_cached_size = nullptr;
 
 // A plain strided CUDA tensor with memory of its own, contiguous, of this type; null for anything else.
 const at::Tensor* plain(PyObject* o, at::ScalarType dtype) {
@@ -181,6 +188,167 @@ PyObject* fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the paged cache -------------------------------------------------------------------------------------------------------------
+// An int that is one and fits 32 bits, or false.
+bool int32_of(PyObject* o, int32_t* v) {
+    if (!PyLong_CheckExact(o)) return false;
+    int overflow = 0;
+    const long long x = PyLong_AsLongLongAndOverflow(o, &overflow);
+    if (overflow || x < INT32_MIN || x > INT32_MAX) return false;
+    *v = static_cast<int32_t>(x);
+    return true;
+}
+// (values, scales) of a cache on q's device, or false.
+struct CacheIn {
+    const at::Tensor *values, *scales;
+};
+bool cache_of(PyObject* o, c10::DeviceIndex device, CacheIn* c) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) return false;
+    c->values = plain(PyTuple_GET_ITEM(o, 0), at::kFloat8_e4m3fn);
+    c->scales = plain(PyTuple_GET_ITEM(o, 1), at::kFloat);
+    return c->values && c->scales && c->values->dim() == 3 && c->scales->dim() == 1 && c->values->size(2) == SMLA_D_QK &&
+           c->scales->size(0) == c->values->size(0) && c->values->size(0) <= INT32_MAX && c->values->size(1) <= 128 && c->values->get_device() == device &&
+           c->scales->get_device() == device;
+}
+// [begin, begin + numel of `sizes`) of a buffer of int32 as a tensor of its own.
+at::Tensor part_of(const at::Tensor& buffer, int64_t begin, at::IntArrayRef sizes) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(begin);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
+
+// cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk) -> (slots, query_meta, kv_len, free_count,
+// admitted), a status, or None.
+PyObject* cache_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    smla_cache_plan_params p{};
+    if (n != 8 || !g_cache_plan || !int32_of(a[5], &p.page_size) || !int32_of(a[6], &p.max_tokens) || !int32_of(a[7], &p.topk)) Py_RETURN_NONE;
+    const at::Tensor* t[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = plain(a[i], at::kInt)) || t[i]->get_device() != t[0]->get_device() || t[i]->dim() != (i == 2 ? 2 : 1)) Py_RETURN_NONE;
+    const int64_t requests = t[0]->size(0);
+    if (t[1]->size(0) != requests || t[2]->size(0) != requests || t[4]->size(0) != 1 || requests > 8192 || t[2]->size(1) > INT32_MAX ||
+        t[3]->size(0) > INT32_MAX || p.max_tokens <= 0 || p.max_tokens >= 1 << 30)
+        Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(t[0]->device());
+    // one allocation: query_meta (16-byte aligned), slots, kv_len, admitted, free_count
+    const int64_t T = p.max_tokens;
+    const at::Tensor buffer = empty({5 * T + 2 * requests + 1}, at::kInt, *t[0]);
+    int32_t* out = static_cast<int32_t*>(buffer.data_ptr());
+    p.kv_len = static_cast<const int32_t*>(t[0]->data_ptr());
+    p.new_len = static_cast<const int32_t*>(t[1]->data_ptr());
+    p.block_table = static_cast<int32_t*>(t[2]->data_ptr());
+    p.free_pages = static_cast<int32_t*>(t[3]->data_ptr());
+    p.free_count = static_cast<const int32_t*>(t[4]->data_ptr());
+    p.query_meta = out;
+    p.slots = out + 4 * T;
+    p.kv_len_out = out + 5 * T;
+    p.admitted = out + 5 * T + requests;
+    p.free_count_out = out + 5 * T + 2 * requests;
+    p.n_requests = static_cast<int32_t>(requests);
+    p.max_pages = static_cast<int32_t>(t[2]->size(1));
+    p.n_free = static_cast<int32_t>(t[3]->size(0));
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(t[0]->get_device()).stream();
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_cache_plan(&p, stream);
+    Py_END_ALLOW_THREADS
+    if (st != SMLA_OK) return PyLong_FromLong(st);
+    const at::Tensor parts[5] = {part_of(buffer, 4 * T, {T}), part_of(buffer, 0, {T, 4}), part_of(buffer, 5 * T, {requests}),
+                                 part_of(buffer, 5 * T + 2 * requests, {1}), part_of(buffer, 5 * T + requests, {requests})};
+    auto result = py::reinterpret_steal<py::object>(PyTuple_New(5));
+    if (!result) return nullptr;
+    for (int i = 0; i < 5; ++i) {
+        PyObject* o = THPVariable_Wrap(parts[i]);
+        if (!o) return nullptr;
+        PyTuple_SET_ITEM(result.ptr(), i, o);
+    }
+    return result.release().ptr();
+    END_HANDLE_TH_ERRORS
+}
+
+// cache_append(kv, cache, slots) -> a status, or None.  (kv contiguous; a strided one goes the other way.)
+PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3 || !g_cache_append || !g_append_size) Py_RETURN_NONE;
+    const at::Tensor *kv = plain(a[0], at::kBFloat16), *slots = plain(a[2], at::kInt);
+    CacheIn c;
+    if (!kv || !slots || kv->dim() != 2 || kv->size(1) != SMLA_D_QK || slots->dim() != 1 || slots->size(0) != kv->size(0) || kv->size(0) > INT32_MAX ||
+        slots->get_device() != kv->get_device() || !cache_of(a[1], kv->get_device(), &c))
+        Py_RETURN_NONE;
+    smla_cache_append_params p{};
+    p.n_rows = static_cast<int32_t>(kv->size(0));
+    const c10::cuda::CUDAGuard guard(kv->device());
+    const size_t need = g_append_size(p.n_rows);
+    at::Tensor ws;
+    if (need) ws = empty({static_cast<int64_t>(need)}, at::kByte, *kv);
+    p.kv = kv->data_ptr();
+    p.slots = static_cast<const int32_t*>(slots->data_ptr());
+    p.values = c.values->data_ptr();
+    p.scales = static_cast<float*>(c.scales->data_ptr());
+    p.kv_stride = SMLA_D_QK;
+    p.n_pages = static_cast<int32_t>(c.values->size(0));
+    p.page_size = static_cast<int32_t>(c.values->size(1));
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(kv->get_device()).stream();
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_cache_append(&p, need ? ws.data_ptr() : nullptr, need, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+    END_HANDLE_TH_ERRORS
+}
+
+// fwd_cached(q, cache, block_table, indices, query_meta, sm_scale, causal, lse_is_base2) -> (o, lse), a status, or None.
+PyObject* fwd_cached(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    smla_fwd_cached_params p{};
+    int32_t unused;
+    if (n != 8 || !g_cached_run || !g_cached_size || !scalars(a[5], Py_None, &p.sm_scale, &unused)) Py_RETURN_NONE;
+    const at::Tensor *q = plain(a[0], at::kBFloat16), *table = plain(a[2], at::kInt), *idx = plain(a[3], at::kInt), *meta = plain(a[4], at::kInt);
+    if (!q || !table || !idx || !meta || q->dim() != 3 || q->size(2) != SMLA_D_QK || table->dim() != 2 || meta->dim() != 2 || meta->size(1) != 4 ||
+        idx->dim() < 2 || idx->dim() > 3 || (idx->dim() == 3 && idx->size(1) != 1))
+        Py_RETURN_NONE;
+    const int64_t s_q = q->size(0), h_q = q->size(1);
+    CacheIn c;
+    if (idx->size(0) != s_q || meta->size(0) != s_q || s_q > INT32_MAX || h_q > 128 || h_q % 8 != 0 || idx->size(-1) > INT32_MAX || table->size(0) > INT32_MAX ||
+        table->size(1) > INT32_MAX || table->get_device() != q->get_device() || idx->get_device() != q->get_device() || meta->get_device() != q->get_device() ||
+        !cache_of(a[1], q->get_device(), &c))
+        Py_RETURN_NONE;
+    const long causal = PyLong_AsLong(a[6]), base2 = PyLong_AsLong(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    p.s_q = static_cast<int32_t>(s_q);
+    p.h_q = static_cast<int32_t>(h_q);
+    p.topk = static_cast<int32_t>(idx->size(-1));
+    p.n_pages = static_cast<int32_t>(c.values->size(0));
+    p.page_size = static_cast<int32_t>(c.values->size(1));
+    p.n_requests = static_cast<int32_t>(table->size(0));
+    p.max_pages = static_cast<int32_t>(table->size(1));
+    p.query_meta = static_cast<const int32_t*>(meta->data_ptr());
+    const size_t need = g_cached_size(&p, 0);
+    if (!need) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(q->device());
+    const at::Tensor o = empty({s_q, h_q, SMLA_D_V}, at::kBFloat16, *q), lse = empty({s_q, h_q}, at::kFloat, *q);
+    const at::Tensor ws = empty({static_cast<int64_t>(need)}, at::kByte, *q);
+    p.q = q->data_ptr();
+    p.values = c.values->data_ptr();
+    p.scales = static_cast<const float*>(c.scales->data_ptr());
+    p.block_table = static_cast<const int32_t*>(table->data_ptr());
+    p.indices = static_cast<const int32_t*>(idx->data_ptr());
+    p.o = o.data_ptr();
+    p.lse = static_cast<float*>(lse.data_ptr());
+    p.causal = causal ? 1 : 0;
+    p.lse_is_base2 = base2 ? 1 : 0;
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(q->get_device()).stream();
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_cached_run(&p, ws.data_ptr(), need, stream);
+    Py_END_ALLOW_THREADS
+    if (st != SMLA_OK) return PyLong_FromLong(st);
+    return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(o)).ptr(), py::reinterpret_steal<py::object>(THPVariable_Wrap(lse)).ptr());
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- Delta = rowsum(O * dO) on the host, for inputs that lie there (smla_host_delta.h) ------------------------------------------
 // O is needed for Delta alone, and Delta is 256 times smaller: found here, O does not have to cross PCIe (29 % of the input bytes of 128
 // heads x 512 columns).  Bound by reading O and dO from the host's memory.
@@ -280,19 +448,25 @@ PyObject* delta_wait(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// init(addresses of smla_fwd_run, smla_fwd_workspace_size, smla_bwd_run_stages, smla_bwd_workspace_size)
+// init(addresses of smla_fwd_run, smla_fwd_workspace_size, smla_bwd_run_stages, smla_bwd_workspace_size, smla_cache_plan, smla_cache_append,
+// smla_cache_append_workspace_size, smla_fwd_cached_run, smla_fwd_cached_workspace_size)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    void* f[4];
-    if (n != 4) {
-        PyErr_SetString(PyExc_TypeError, "init takes four addresses");
+    void* f[9];
+    if (n != 9) {
+        PyErr_SetString(PyExc_TypeError, "init takes nine addresses");
         return nullptr;
     }
-    for (int i = 0; i < 4; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
+    for (int i = 0; i < 9; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
     g_fwd_run = reinterpret_cast<decltype(g_fwd_run)>(f[0]);
     g_fwd_size = reinterpret_cast<decltype(g_fwd_size)>(f[1]);
     g_bwd_run = reinterpret_cast<decltype(g_bwd_run)>(f[2]);
     g_bwd_size = reinterpret_cast<decltype(g_bwd_size)>(f[3]);
+    g_cache_plan = reinterpret_cast<decltype(g_cache_plan)>(f[4]);
+    g_cache_append = reinterpret_cast<decltype(g_cache_append)>(f[5]);
+    g_append_size = reinterpret_cast<decltype(g_append_size)>(f[6]);
+    g_cached_run = reinterpret_cast<decltype(g_cached_run)>(f[7]);
+    g_cached_size = reinterpret_cast<decltype(g_cached_size)>(f[8]);
     Py_RETURN_NONE;
 }
 
@@ -301,6 +475,9 @@ PyMethodDef g_methods[] = {{"init", fast<init>(), METH_FASTCALL, nullptr},
                            {"fwd", fast<fwd>(), METH_FASTCALL, nullptr},
                            {"bwd_need", fast<bwd_need>(), METH_FASTCALL, nullptr},
                            {"bwd", fast<bwd>(), METH_FASTCALL, nullptr},
+                           {"cache_plan", fast<cache_plan>(), METH_FASTCALL, nullptr},
+                           {"cache_append", fast<cache_append>(), METH_FASTCALL, nullptr},
+                           {"fwd_cached", fast<fwd_cached>(), METH_FASTCALL, nullptr},
                            {"delta_start", fast<delta_start>(), METH_FASTCALL, nullptr},
                            {"delta_wait", fast<delta_wait>(), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};

@@ -210,6 +210,18 @@ class _NoNativeHost:
         return None
 
     @staticmethod
+    def cache_plan(*_):
+        return None
+
+    @staticmethod
+    def cache_append(*_):
+        return None
+
+    @staticmethod
+    def fwd_cached(*_):
+        return None
+
+    @staticmethod
     def delta_start(*_):
         return None
 
@@ -241,7 +253,8 @@ def _load_host(lib):
         module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_smla_host", loader, origin=path))
         loader.exec_module(module)
         module.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in
-                      (lib.smla_fwd_run, lib.smla_fwd_workspace_size, lib.smla_bwd_run_stages, lib.smla_bwd_workspace_size)))
+                      (lib.smla_fwd_run, lib.smla_fwd_workspace_size, lib.smla_bwd_run_stages, lib.smla_bwd_workspace_size, lib.smla_cache_plan,
+                       lib.smla_cache_append, lib.smla_cache_append_workspace_size, lib.smla_fwd_cached_run, lib.smla_fwd_cached_workspace_size)))
         return module
     except Exception as e:
         warnings.warn(f"the compiled host module cannot be used, calls take some 10 us longer: {e}")
@@ -768,6 +781,9 @@ def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.T
     size for a step that is captured in a graph), have slot -1 and an empty query.  Requests are served in order; one for which the pages, the
     table's width or the rows do not suffice gets nothing in this step (`admitted` 0, its rows' slots -1), nor does a later one that needs a
     page once there were too few.  At most 8192 requests; nothing synchronises."""
+    out = _host().cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk)
+    if type(out) is tuple:
+        return CachePlan._make(out)
     _check(isinstance(kv_len, torch.Tensor) and kv_len.is_cuda, "kv_len must be a CUDA tensor")
     device = kv_len.device
     _check_int32(kv_len, (None,), device, "kv_len")
@@ -801,6 +817,8 @@ def cache_append(kv: torch.Tensor, cache: LatentCache, slots: torch.Tensor) -> N
     smallest power of two (2^-100 at least) that holds the rows it gets now.  Any other page's scale grows where they need it, and the rows
     it keeps are brought over.  Of several rows with one slot the last one is kept; slots may come in any order, and ones outside the cache
     are left out.  A number that is not finite is stored as a NaN.  Enqueues on the current stream; calls on one cache must be ordered."""
+    if _host().cache_append(kv, cache, slots) == 0:
+        return
     _check(isinstance(kv, torch.Tensor) and kv.is_cuda and kv.dtype == torch.bfloat16, "kv must be a bfloat16 CUDA tensor")
     if kv.dim() == 3 and kv.shape[1] == 1:
         kv = kv[:, 0]
@@ -839,6 +857,10 @@ def mla_fwd_cached(q: torch.Tensor, cache: LatentCache, block_table: torch.Tenso
     in use (all int32).  A slot counts if it is in use, its position lies in the request's tokens and, with `causal`, not behind the query's,
     and its page is one of the cache.  A query without such a slot (a padding row) gives o = 0 and lse = +inf.  Of a page's scale the exponent
     is used.  Prompts and single tokens take the same call."""
+    if workspace is None and not (workspace_budget or check_device_status):
+        out = _host().fwd_cached(q, cache, block_table, indices, query_meta, sm_scale, 1 if causal else 0, 1 if lse_is_base2 else 0)
+        if type(out) is tuple:
+            return out
     for name, t in (("q", q), ("indices", indices)):
         _check(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous(), f"{name} must be a contiguous CUDA tensor")
     _check(q.dtype == torch.bfloat16 and indices.dtype == torch.int32, "dtypes: q bfloat16, indices int32")
