@@ -48,6 +48,17 @@ __device__ __forceinline__ void split_e4m3x4(uint64_t x01, uint64_t x23, uint32_
     const float2 e = unpack_f32x2(fma_f32x2(pack_f32x2(c.x, c.y), minus, x01)), f = unpack_f32x2(fma_f32x2(pack_f32x2(d.x, d.y), minus, x23));
     *lo = cvt_e4m3x4(e.x, e.y, f.x, f.y);
 }
+// The same with hi cut off after four significant bits, fewer instructions: exact for numbers of eight bits from 2^-2 on, within half of 2^-9
+// from 2^-6 on, within 2^-9 below (there hi is rounded too).
+__device__ __forceinline__ void split_cut_e4m3x4(uint64_t x01, uint64_t x23, uint32_t* hi, uint32_t* lo) {
+    const float2 a = unpack_f32x2(x01), b = unpack_f32x2(x23);
+    auto cut = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xfff00000u); };
+    const float2 c = make_float2(cut(a.x), cut(a.y)), d = make_float2(cut(b.x), cut(b.y));
+    *hi = cvt_e4m3x4(c.x, c.y, d.x, d.y);
+    const uint64_t minus = pack_f32x2(-1.f, -1.f);
+    const float2 e = unpack_f32x2(fma_f32x2(pack_f32x2(c.x, c.y), minus, x01)), f = unpack_f32x2(fma_f32x2(pack_f32x2(d.x, d.y), minus, x23));
+    *lo = cvt_e4m3x4(e.x, e.y, f.x, f.y);
+}
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
@@ -204,8 +215,10 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
 // The first row of a run (neighbours in the call that name one page) speaks for the run; a page may come up in several runs, whose
 // first one does the work for all.  Up to kAppendDirect rows every row has a block, which looks through the whole slot map; beyond that
 // a first kernel lists the runs, and the blocks go through the list.
-// Bound by HBM (1152 bytes read and 576 written a row) for prompts, by latency for the rows of a decoding step.
-// =============================================================================================
+// Bound by HBM (1152 bytes read and 576 written a row) for prompts, by latency for the rows of a decoding step.  65536 rows in 37 requests, pages
+// of 128: 61 us with a block a page, 42 with two blocks of a cluster that exchange their maxima (2.7 TB/s; the same rows again and again, 36 us).
+// On those: 46 with four blocks, whose lists and tables to look through are the larger part of their instructions, 58 - 65 with the rows held in
+// registers in between, fewer blocks at a time.  Pages of 64 / 32 / 16: 32 / 42 / 96 us, a run's lookups for fewer rows.
 struct CacheAppendArgs {
     const __nv_bfloat16* kv;
     long long kv_stride;          // elements from row to row
@@ -217,10 +230,14 @@ struct CacheAppendArgs {
     int* counts;                  // [lists]
     int n_lists, list_len;
 };
-constexpr int kAppendThreads = 256;
+constexpr int kAppendUnits = kDQK / 8;        // 16 bytes of a bf16 row, 8 bytes of a stored one
+constexpr int kAppendSide = 4;                // rows that a block works on side by side
+constexpr int kAppendThreads = kAppendSide * kAppendUnits;
+static_assert(kAppendThreads % 32 == 0 && kAppendThreads >= kMaxPageRows, "whole warps, a thread for a page's row");
 constexpr int kAppendDirect = 2048;
-constexpr int kAppendListLen = 4096;
+constexpr int kAppendListLen = 1024;
 constexpr int kAppendMaxLists = 512;
+constexpr int kAppendBlockRows = 64;         // rows of a page that a block of the listed form takes
 
 __device__ __forceinline__ int append_page_of(const CacheAppendArgs& a, int slot) {
     const int page = slot >> a.page_shift;
@@ -252,69 +269,91 @@ struct AppendShared {
     uint32_t warp_max[kAppendThreads / 32];
 };
 
-// The page's rows are known (win); quantise and write them.
-__device__ __forceinline__ void append_write_page(const CacheAppendArgs& a, int page, AppendShared& sh) {
-    constexpr int kUnits = kDQK / 8;              // 16 bytes of a bf16 row, 8 bytes of a stored one
-    const int page_rows = 1 << a.page_shift;
-    if (static_cast<int>(threadIdx.x) < page_rows && sh.win[threadIdx.x] >= 0) sh.rows[atomicAdd(&sh.n_rows, 1)] = threadIdx.x;
-    __syncthreads();
-    const int n_units = sh.n_rows * kUnits;
-    auto source = [&](int u) {
-        const int i = u / kUnits;
-        return reinterpret_cast<const uint4*>(a.kv + static_cast<long long>(sh.win[sh.rows[i]]) * a.kv_stride) + (u - i * kUnits);
-    };
-    uint32_t top = 0;                             // largest finite |x|, as the bits of an fp32 number
-#pragma unroll 4
-    for (int u = threadIdx.x; u < n_units; u += kAppendThreads) {
-        const uint4 v = __ldg(source(u));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// The largest magnitude of even and odd columns so far and of eight more, as two sets of bf16 bits.
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t top, const uint4& v) {
+    return __vmaxu2(__vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu)), v.w & 0x7fff7fffu);
+}
+// The same for a page that has seen something not finite: over what is.
+__device__ __forceinline__ uint32_t finite_max_bf16x2(uint32_t top, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = w[k] & 0x7fffu, hi = w[k] & 0x7fff0000u;
+        top = __vmaxu2(top, (lo < 0x7f80u ? lo : 0u) | (hi < 0x7f800000u ? hi : 0u));
+    }
+    return top;
+}
+// Eight columns as they are stored.  An infinity is stored as a NaN: the format has none, and it has no place among finite numbers.
+__device__ __forceinline__ uint2 append_cvt(const uint4& v, float inv, bool all_finite) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint64_t inv2 = pack_f32x2(inv, inv);
+    float2 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)), inv2));
+    if (!all_finite) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint32_t lo = (w[k] << 16) & 0x7fff0000u, hi = w[k] & 0x7fff0000u;
-            top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+            if ((w[k] & 0x7fffu) >= 0x7f80u) x[k].x = __uint_as_float(0x7fffffffu);
+            if ((w[k] & 0x7fff0000u) >= 0x7f800000u) x[k].y = __uint_as_float(0x7fffffffu);
         }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    return make_uint2(cvt_e4m3x4(x[0].x, x[0].y, x[1].x, x[1].y), cvt_e4m3x4(x[2].x, x[2].y, x[3].x, x[3].y));
+}
+// Rows [r0, r1) that the page keeps go over to its new scale.
+__device__ __forceinline__ void append_rescale(const AppendShared& sh, uint8_t* base, int r0, int r1, float ratio) {
+    for (int u = r0 * (kDQK / 16) + threadIdx.x; u < r1 * (kDQK / 16); u += kAppendThreads) {
+        if (sh.win[u / (kDQK / 16)] >= 0) continue;
+        uint4* at = reinterpret_cast<uint4*>(base + static_cast<size_t>(u) * 16);
+        const uint4 v = *at;
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 lo = e4m3x2_to_float2(w[k] & 0xffffu), hi = e4m3x2_to_float2(w[k] >> 16);
+            w[k] = cvt_e4m3x4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+        }
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Largest magnitude that the block's threads have seen, as bf16 bits; in every thread, behind a barrier.
+__device__ __forceinline__ uint32_t append_block_max(uint32_t top, AppendShared& sh) {
+    top = __reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xffffu));
     if ((threadIdx.x & 31) == 0) sh.warp_max[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, sh.warp_max[w]);
-    const float wanted = exp2_int(scale_exp(top));
+    return top;
+}
+
+// The page's rows are known (win); quantise and write them.
+__device__ __forceinline__ void append_write_page(const CacheAppendArgs& a, int page, AppendShared& sh) {
+    const int page_rows = 1 << a.page_shift;
+    if (static_cast<int>(threadIdx.x) < page_rows && sh.win[threadIdx.x] >= 0) sh.rows[atomicAdd(&sh.n_rows, 1)] = threadIdx.x;
     const float old = a.scales[page];
+    __syncthreads();
+    const int slot = threadIdx.x / kAppendUnits, unit = threadIdx.x % kAppendUnits, n = sh.n_rows;
+    auto source = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(a.kv + static_cast<long long>(sh.win[sh.rows[i]]) * a.kv_stride) + unit); };
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int i = slot; i < n; i += kAppendSide) top = max_bf16x2(top, source(i));
+    top = append_block_max(top, sh);
+    const bool all_finite = top < 0x7f80u;
+    if (!all_finite) {
+        top = 0;
+        __syncthreads();
+        for (int i = slot; i < n; i += kAppendSide) top = finite_max_bf16x2(top, source(i));
+        top = append_block_max(top, sh);
+    }
+    const float wanted = exp2_int(scale_exp(top << 16));
     const bool anew = sh.win[0] >= 0;             // its first row is written: what it held belongs to nobody
     const float scale = anew ? wanted : fmaxf(old, wanted);
-    __syncthreads();                              // (the old scale has been read)
     uint8_t* base = a.values + static_cast<size_t>(page) * page_rows * kDQK;
-    if (!anew && scale > old) {
-        const float ratio = old / scale;
-        for (int u = threadIdx.x; u < page_rows * (kDQK / 16); u += kAppendThreads) {
-            const int r = u / (kDQK / 16);
-            if (sh.win[r] >= 0) continue;
-            uint4* at = reinterpret_cast<uint4*>(base + static_cast<size_t>(u) * 16);
-            const uint4 v = *at;
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 lo = e4m3x2_to_float2(w[k] & 0xffffu), hi = e4m3x2_to_float2(w[k] >> 16);
-                w[k] = cvt_e4m3x2(lo.x * ratio, lo.y * ratio) | cvt_e4m3x2(hi.x * ratio, hi.y * ratio) << 16;
-            }
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
+    if (!anew && scale > old) append_rescale(sh, base, 0, page_rows, old / scale);
     if (threadIdx.x == 0) a.scales[page] = scale;
     const float inv = 1.f / scale;
-    // an infinity is stored as a NaN: the format has none, and it has no place among finite numbers
-    auto scaled = [&](uint32_t bits) { return (bits & 0x7fffffffu) < 0x7f800000u ? __uint_as_float(bits) * inv : __uint_as_float(0x7fffffffu); };
 #pragma unroll 4
-    for (int u = threadIdx.x; u < n_units; u += kAppendThreads) {
-        const uint4 v = __ldg(source(u));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t c[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) c[k] = cvt_e4m3x2(scaled(w[k] << 16), scaled(w[k] & 0xffff0000u));
-        const int i = u / kUnits;
-        *reinterpret_cast<uint2*>(base + static_cast<size_t>(sh.rows[i]) * kDQK + (u - i * kUnits) * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-    }
+    for (int i = slot; i < n; i += kAppendSide)
+        *reinterpret_cast<uint2*>(base + static_cast<size_t>(sh.rows[i]) * kDQK + unit * 8) = append_cvt(source(i), inv, all_finite);
 }
 
 __device__ __forceinline__ void append_clear(AppendShared& sh) {
@@ -344,10 +383,14 @@ __global__ void __launch_bounds__(kAppendThreads) smla_cache_append_kernel(const
     append_write_page(a, page, sh);
 }
 
-__global__ void __launch_bounds__(kAppendThreads) smla_cache_append_listed_kernel(const CacheAppendArgs a) {
+// The blocks of a cluster share a page, 64 rows each.  They read them twice, the second time out of the L2: what holds them in between (32
+// registers a thread) halves the blocks that are in place on an SM, and a page's way is a chain of a dozen latencies.
+__global__ void __launch_bounds__(kAppendThreads, 6) smla_cache_append_listed_kernel(const CacheAppendArgs a) {
     __shared__ AppendShared sh;
     __shared__ int before[kAppendMaxLists + 1];   // runs in the lists before
-    const int row_mask = (1 << a.page_shift) - 1;
+    __shared__ __align__(16) uint32_t page_max[2][4];            // [parity of the page]
+    const int row_mask = (1 << a.page_shift) - 1, page_rows = row_mask + 1;
+    const int n_blocks = cluster_nctas(), rank = cluster_ctarank();
     pdl_wait();
     pdl_trigger();
     if (threadIdx.x < 32) {
@@ -371,11 +414,15 @@ __global__ void __launch_bounds__(kAppendThreads) smla_cache_append_listed_kerne
         const int l = last_not_above(before, a.n_lists, g);
         return __ldcg(a.runs + static_cast<size_t>(l) * a.list_len + (g - before[l]));
     };
-    for (int item = blockIdx.x; item < n_runs; item += gridDim.x) {
+    int parity = 0;
+    for (int item = blockIdx.x / n_blocks; item < n_runs; item += gridDim.x / n_blocks) {
         const int2 mine = run(item);
+        if (threadIdx.x == 0) sh.end = a.n_rows;
         append_clear(sh);
         auto take = [&](int t) { atomicMax(&sh.win[__ldg(a.slots + t) & row_mask], t); };
         auto in_run = [&](int t) { return t < a.n_rows && append_page_of(a, __ldg(a.slots + t)) == mine.x; };
+        if (!in_run(mine.y + threadIdx.x)) atomicMin(&sh.end, mine.y + static_cast<int>(threadIdx.x));
+#pragma unroll 2
         for (int g = threadIdx.x; g < n_runs; g += kAppendThreads) {
             const int2 other = run(g);
             if (other.x != mine.x || other.y == mine.y) continue;
@@ -384,22 +431,62 @@ __global__ void __launch_bounds__(kAppendThreads) smla_cache_append_listed_kerne
                 for (int t = other.y; in_run(t); ++t) take(t);         // (seldom: the page comes up again)
         }
         __syncthreads();
-        if (!sh.earlier) {
-            for (int t0 = mine.y;; t0 += kAppendThreads) {
-                if (threadIdx.x == 0) sh.end = a.n_rows;
-                __syncthreads();
-                const int t = t0 + threadIdx.x;
-                if (!in_run(t)) atomicMin(&sh.end, t);
-                __syncthreads();
-                const int end = sh.end;
+        if (!sh.earlier) {                        // (alike in all blocks of the cluster)
+            int t0 = mine.y;
+            while (true) {                        // (once, unless slots are named twice)
+                const int t = t0 + static_cast<int>(threadIdx.x), end = sh.end;
                 if (t < end) take(t);
                 __syncthreads();
-                if (end < t0 + kAppendThreads) break;
+                t0 += kAppendThreads;
+                if (end < t0 || t0 >= a.n_rows) break;
+                if (threadIdx.x == 0) sh.end = a.n_rows;
+                __syncthreads();
+                if (!in_run(t0 + threadIdx.x)) atomicMin(&sh.end, t0 + static_cast<int>(threadIdx.x));
+                __syncthreads();
             }
-            append_write_page(a, mine.x, sh);
+            // this block's rows of the page
+            const int r0 = rank * kAppendBlockRows, r1 = min(r0 + kAppendBlockRows, page_rows);
+            const int r = r0 + static_cast<int>(threadIdx.x);
+            if (r < r1 && sh.win[r] >= 0) sh.rows[atomicAdd(&sh.n_rows, 1)] = r;
+            const float old = __ldcg(a.scales + mine.x);
+            __syncthreads();
+            const int slot = threadIdx.x / kAppendUnits, unit = threadIdx.x % kAppendUnits, n = sh.n_rows;
+            auto source = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(a.kv + static_cast<long long>(sh.win[sh.rows[i]]) * a.kv_stride) + unit); };
+            uint32_t top = 0, finite;
+#pragma unroll 4
+            for (int i = slot; i < n; i += kAppendSide) top = max_bf16x2(top, source(i));
+            top = finite = append_block_max(top, sh);
+            if (top >= 0x7f80u) {
+                finite = 0;
+                __syncthreads();
+                for (int i = slot; i < n; i += kAppendSide) finite = finite_max_bf16x2(finite, source(i));
+                finite = append_block_max(finite, sh);
+            }
+            if (threadIdx.x == 0) *reinterpret_cast<uint2*>(page_max[parity]) = make_uint2(top, finite);
+            cluster_sync_all();
+            uint32_t tops[4], finites[4];         // (the first again where there are fewer blocks)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 other = ld_cluster_v4(map_to_cta(smem_u32(page_max[parity]), k < n_blocks ? k : 0));
+                tops[k] = __float_as_uint(other.x);
+                finites[k] = __float_as_uint(other.y);
+            }
+            top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+            finite = max(max(finites[0], finites[1]), max(finites[2], finites[3]));
+            parity ^= 1;                          // (the next page's sync comes before this place is written again)
+            const bool anew = sh.win[0] >= 0;
+            const float wanted = exp2_int(scale_exp(finite << 16)), scale = anew ? wanted : fmaxf(old, wanted);
+            uint8_t* base = a.values + static_cast<size_t>(mine.x) * page_rows * kDQK;
+            if (!anew && scale > old) append_rescale(sh, base, r0, r1, old / scale);
+            if (threadIdx.x == 0 && rank == 0) a.scales[mine.x] = scale;
+            const float inv = 1.f / scale;
+#pragma unroll 4
+            for (int i = slot; i < n; i += kAppendSide)
+                *reinterpret_cast<uint2*>(base + static_cast<size_t>(sh.rows[i]) * kDQK + unit * 8) = append_cvt(source(i), inv, top < 0x7f80u);
         }
         __syncthreads();                          // (the next page's tables go to the same place)
     }
+    cluster_sync_all();                           // (nobody leaves while another may read its maximum)
 }
 
 }  // namespace smla
