@@ -111,7 +111,7 @@ def attend_ref(q, values, scales, block_table, indices, query_meta, sm_scale=Non
     """In 64 bits, query by query, on q's device, with bounds on what the roundings of the product path can amount to:
 
     logits   fp32 sums of 576 products (2 x 576 with q in two parts): 2^-18 of the sum of magnitudes covers their alignment to the largest
-             one in every step (probed: 2.5e-6 where one product dominates); q within half of a step of 2^-9 where its row's largest magnitude is 224 to 448.
+             one in every step (probed: 2.5e-6 where one product dominates); q within 2^-9 (both parts rounded) where its row's largest magnitude is 224 to 448.
     P        half a step of eight significant bits, 2^-8, and half of 2^-9 where the largest P of the row is 64 to 256: 2^-16 of the largest.
     o        half a step of bf16, 2^-8.   ex2, the division and the sums in fp32: a few 2^-22.
     log2 s   is added to the logits and taken out again by way of the sum's logarithm: numbers of size |log2 s|, each of three roundings half of
@@ -143,7 +143,7 @@ def attend_ref(q, values, scales, block_table, indices, query_meta, sm_scale=Non
         out.lse[i] = torch.logsumexp(logits, 1) / math.log(2)
         p = torch.softmax(logits, 1)
         out.o[i] = p @ k[:, :D_V]
-        size = (x.abs() @ k.abs().T * 2.0 ** -18 + x.abs().amax(1, keepdim=True) * k.abs().sum(1) * 2.0 ** -10 / 224) * abs(sm_scale)
+        size = (x.abs() @ k.abs().T * 2.0 ** -18 + x.abs().amax(1, keepdim=True) * k.abs().sum(1) * 2.0 ** -9 / 224) * abs(sm_scale)
         off = size.amax(1, keepdim=True) + 2.0 ** -20 + logits.abs().amax(1, keepdim=True) * 2.0 ** -22 + float(s.log2().abs().max()) * 2.0 ** -24
         heavy = (p * s[:, 0]).amax(1, keepdim=True)
         out.o_bound[i] = (2.0 ** -8 + 2 * off) * (p @ k[:, :D_V].abs()) + 2.0 ** -16 * heavy * code[:, :D_V].abs().sum(0) + 2.0 ** -8 * out.o[i].abs()

@@ -5,8 +5,8 @@
 //   operands   kind::f8f6f4 UMMAs on the stored e4m3 numbers as they lie, for K and for V: nothing is converted on the way, and a
 //              gathered row is 576 bytes instead of 1152.  The other side of either product is the sum of two e4m3 numbers, one UMMA each:
 //              q = 2^e (hi + lo) with e from the row's largest magnitude.  A bf16 number has eight significant bits; hi takes four,
-//              what it leaves has four at most, so hi + lo is q exactly for what is within 2^-10 of the row's largest, and within half of
-//              2^-9, 2^-17.8 of the largest, for the rest.  P hi + lo likewise: within 2^-9 of P, bf16's is 2^-8, and within half of 2^-9.
+//              lo the other four, so hi + lo is q exactly for what is within 2^-10 of the row's largest, and within 2^-16.8 of the largest
+//              for the rest.  P hi + lo, hi rounded to the nearest: within 2^-9 of P, bf16's is 2^-8, and within half of 2^-9 below 2^-2.
 //              An 8-bit UMMA takes 32 of K in the time of 16 in bf16, so two of them cost what one contraction in bf16 costs.
 //   scales     of a key's page, s_j.  The logits are x_j = scale 2^e s_j (hi + lo) c_j.  V needs p_j s_j, and that is what is rounded:
 //              P_j = 2^(x_j + log2 s_j - ref), so that the heaviest P_j are alike whatever the pages' scales are: with ref set the
@@ -100,8 +100,8 @@ __device__ __noinline__ void split_row(const __nv_bfloat16* row, uint32_t image,
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = mul_f32x2(pack_f32x2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)), f2);
         uint32_t h[2], l[2];
-        split_e4m3x4(x[0], x[1], &h[0], &l[0]);
-        split_e4m3x4(x[2], x[3], &h[1], &l[1]);
+        split_cut_e4m3x4(x[0], x[1], &h[0], &l[0]);
+        split_cut_e4m3x4(x[2], x[3], &h[1], &l[1]);
         const int unit = (j & 1) * 4 + (u >> 1);
         const uint32_t to_hi = to + (j >> 1) * 2 * kTerm + ((unit ^ (r & 7)) << 4);
         const uint32_t to_lo = j < 8 ? to_hi + kTerm : to + 8 * kTerm + (((4 + unit) ^ (r & 7)) << 4);
