@@ -4,6 +4,9 @@
 // The cache: values e4m3 [n_pages][page rows][576], scales fp32 [n_pages].  A page's rows share one scale, a power of two, so that going
 // over to a larger scale moves exponents only (a number rounds again only where it becomes subnormal), and so that a stored number
 // times its scale is a bf16 number exactly.  A slot is page * page rows + row.
+//
+// These kernels and the forward may come up under one another's tails.  What one of them changes in place (tables, free pages, scales, values)
+// is read past the L1: a line of it that a block of the kernel before has brought there need not hold what another block of that kernel wrote.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -177,9 +180,9 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.free_count_out = min(stack - n_taken, a.n_free);
     // place s of the stack of free pages, the pages given back on top
     auto stacked = [&](int s) {
-        if (s < n_free) return __ldg(a.free_pages + s);
+        if (s < n_free) return __ldcg(a.free_pages + s);
         const int v = s - n_free, i = last_not_above(backx, a.n_req, v);
-        return __ldg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
+        return __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
     };
     const int at = blockIdx.x * kCachePlanThreads + threadIdx.x, step = gridDim.x * kCachePlanThreads;
     for (int t = at; t < a.max_tokens; t += step) {
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
             const int i = last_not_above(first, a.n_req, t), old = len[i];
             if (old >= 0) {
                 const int pos = old + t - first[i], k = pos >> a.page_shift, have = pages_of(old);
-                const int pg = k < have ? __ldg(a.table + static_cast<size_t>(i) * a.max_pages + k) : stacked(stack - 1 - (needx[i] + k - have));
+                const int pg = k < have ? __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + k) : stacked(stack - 1 - (needx[i] + k - have));
                 slot = pg * page + (pos & (page - 1));
                 m = make_int4(i, old + (first[i + 1] - first[i]), pos, a.topk);
             }
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
     }
     for (int v = at; v < n_back && n_free + v < a.n_free; v += step) {
         const int i = last_not_above(backx, a.n_req, v);
-        a.free_pages[n_free + v] = __ldg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
+        a.free_pages[n_free + v] = __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
     }
 }
 
@@ -304,7 +307,7 @@ __device__ __forceinline__ void append_rescale(const AppendShared& sh, uint8_t* 
     for (int u = r0 * (kDQK / 16) + threadIdx.x; u < r1 * (kDQK / 16); u += kAppendThreads) {
         if (sh.win[u / (kDQK / 16)] >= 0) continue;
         uint4* at = reinterpret_cast<uint4*>(base + static_cast<size_t>(u) * 16);
-        const uint4 v = *at;
+        const uint4 v = __ldcg(at);
         uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -329,7 +332,7 @@ __device__ __forceinline__ uint32_t append_block_max(uint32_t top, AppendShared&
 __device__ __forceinline__ void append_write_page(const CacheAppendArgs& a, int page, AppendShared& sh) {
     const int page_rows = 1 << a.page_shift;
     if (static_cast<int>(threadIdx.x) < page_rows && sh.win[threadIdx.x] >= 0) sh.rows[atomicAdd(&sh.n_rows, 1)] = threadIdx.x;
-    const float old = a.scales[page];
+    const float old = __ldcg(a.scales + page);
     __syncthreads();
     const int slot = threadIdx.x / kAppendUnits, unit = threadIdx.x % kAppendUnits, n = sh.n_rows;
     auto source = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(a.kv + static_cast<long long>(sh.win[sh.rows[i]]) * a.kv_stride) + unit); };

@@ -39,7 +39,7 @@ struct CacheView {
 __device__ __forceinline__ int cached_page(const CacheView& c, int idx, int key, const QMeta& m, int causal) {
     const bool ok = key < m.topk_len && idx >= 0 && idx < m.kv_len && (!causal || idx <= m.q_pos) && m.kv_base >= 0 && m.kv_base < c.n_req &&
                     (idx >> c.page_shift) < c.max_pages;
-    return ok ? __ldg(c.table + static_cast<size_t>(m.kv_base) * c.max_pages + (idx >> c.page_shift)) : -1;
+    return ok ? __ldcg(c.table + static_cast<size_t>(m.kv_base) * c.max_pages + (idx >> c.page_shift)) : -1;
 }
 
 namespace fc {
@@ -264,7 +264,7 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
                     valid[i] = page[i] >= 0 && page[i] < c.n_pages;
                     st_shared_s32(mine + (key >> 7) * 512 + key % kRows * (kCopies * 4) + key / kRows % kCopies * 4,
                                   valid[i] ? (page[i] << c.page_shift) + at_row[i] : -1);
-                    scale[i] = valid[i] ? __ldg(c.scales + page[i]) : 1.f;
+                    scale[i] = valid[i] ? __ldcg(c.scales + page[i]) : 1.f;
                 }
                 slots_next = slots_page;
                 load_page();
