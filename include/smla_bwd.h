@@ -176,7 +176,7 @@ int smla_fwd_run(const smla_fwd_params* p, void* workspace, size_t workspace_byt
  *   query_meta i32 [max_tokens][4]   {request, its tokens after the step, the token's position, topk}; zeros where the slot is -1
  * free_pages [n_free] (the stack: entries below *free_count are free) and block_table are updated in place; kv_len_out, free_count_out
  * and admitted (tokens) are written; kv_len, new_len and free_count are not changed, so a call made twice does the same again.
- * At most 8192 requests.  max_tokens may be 0 (a step that only ends requests); slots and query_meta may be null then. */
+ * The outputs must not be inputs.  At most 8192 requests.  max_tokens may be 0 (a step that only ends requests); slots and query_meta may be null then. */
 typedef struct smla_cache_plan_params {
     const int32_t* kv_len;      /* [n_requests] tokens in the cache */
     const int32_t* new_len;     /* [n_requests] */
