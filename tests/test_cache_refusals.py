@@ -34,16 +34,16 @@ def _append(workspace=A, workspace_bytes=1 << 30, **changes):
 
 @pytest.mark.parametrize("changes", [
     {"kv": 0}, {"kv": A + 8}, {"slots": 0}, {"values": 0}, {"values": A + 4}, {"scales": 0}, {"kv_stride": 580}, {"kv_stride": -576}, {"n_rows": 0},
-    {"n_rows": -1}, {"n_pages": 0}, {"page_size": 63}, {"n_pages": 1 << 25}, {"n_rows": 5000, "workspace": None}, {"n_rows": 5000, "workspace": A + 16}])
+    {"n_rows": -1}, {"n_pages": 0}, {"page_size": 63}, {"n_pages": 1 << 25}, {"n_rows": 9000, "workspace": None}, {"n_rows": 9000, "workspace": A + 16}])
 def test_append_refuses(changes):
     assert _append(**changes) == BAD
 
 
 def test_append_asks_for_its_workspace():
     lib = op.load_library()
-    assert lib.smla_cache_append_workspace_size(2048) == 0
-    need = lib.smla_cache_append_workspace_size(5000)
-    assert need >= 5000 * 8 and _append(n_rows=5000, workspace_bytes=need - 1) == WORKSPACE
+    assert lib.smla_cache_append_workspace_size(8192) == 0
+    need = lib.smla_cache_append_workspace_size(9000)
+    assert need >= 9000 * 8 and _append(n_rows=9000, workspace_bytes=need - 1) == WORKSPACE
 
 
 def _cached(workspace=A, workspace_bytes=1 << 30, **changes):

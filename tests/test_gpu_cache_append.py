@@ -45,7 +45,7 @@ def test_single_tokens(n, page):
 
 
 @pytest.mark.parametrize("page", [16, 64, 128])
-@pytest.mark.parametrize("n", [2047, 2048, 2049, 4097, 9000])
+@pytest.mark.parametrize("n", [2047, 8192, 8193, 9000, 20001])
 def test_prompts(n, page):
     # runs of tokens that begin and end inside pages, some rows left out, the last ones behind the end
     rng = np.random.default_rng(n + page)
@@ -69,7 +69,7 @@ def test_prompts(n, page):
     _check(_kv(n, page), values, scales, slots)
 
 
-@pytest.mark.parametrize("n", [300, 3000, 9001])
+@pytest.mark.parametrize("n", [300, 3000, 9001, 20011])
 def test_any_order_and_slots_named_twice(n):
     # pages come up again and again, slots twice and more often (the last row stays), numbers outside the cache are left out
     rng = np.random.default_rng(n)
@@ -81,7 +81,7 @@ def test_any_order_and_slots_named_twice(n):
     _check(_kv(n, 2), values, scales, slots)
 
 
-@pytest.mark.parametrize("n", [500, 5000])
+@pytest.mark.parametrize("n", [500, 5000, 9000])
 def test_every_row_to_one_slot(n):
     values, scales = random_cache(3, 64, DEV)
     _check(_kv(n, 3), values, scales, [64 + 5] * n)
@@ -160,17 +160,39 @@ def test_pages_behind_two_to_the_32_bytes():
     assert not cache.values[:n_pages - 100].view(torch.uint8).any()
 
 
-def test_replayed_in_a_graph():
+@pytest.mark.parametrize("n", [5000, 9000])
+def test_replayed_in_a_graph(n):
     from test_operator_b200 import op
-    kv, slots = _kv(5000, 7).to(DEV), on(DEV, np.random.default_rng(1).permutation(6400)[:5000].astype(np.int32))[0]
-    cache = op.LatentCache.empty(100, 64, DEV)
+    kv, slots = _kv(n, 7).to(DEV), on(DEV, np.random.default_rng(1).permutation(12800)[:n].astype(np.int32))[0]
+    cache = op.LatentCache.empty(200, 64, DEV)
     op.cache_append(kv, cache, slots)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         op.cache_append(kv, cache, slots)
-    kv.copy_(_kv(5000, 8).to(DEV))
+    kv.copy_(_kv(n, 8).to(DEV))
     again = op.LatentCache(cache.values.clone(), cache.scales.clone())
     graph.replay()
     op.cache_append(kv, again, slots)
     torch.cuda.synchronize()
     assert torch.equal(cache.values.view(torch.uint8), again.values.view(torch.uint8)) and torch.equal(cache.scales, again.scales)
+
+
+@pytest.mark.parametrize("n", [64, 9000])
+def test_calls_queued_one_behind_the_other(n):
+    # nothing between the calls: a later one may come up under an earlier one's tail, on the same pages
+    from test_operator_b200 import op
+    page, calls = 16, 12
+    pages = -(-n // 8)
+    cache = op.LatentCache.empty(pages, page, DEV)
+    want_v, want_s = np.zeros((pages, page, 576)), np.zeros(pages)
+    kvs, slot_maps = [], []
+    for k in range(calls):
+        kvs.append(_kv(n, k, grow=0) * float(2.0 ** (k % 5)))
+        slot_maps.append(np.array([(t // 8) * page + (t + k) % 8 + (8 if k % 2 else 0) for t in range(n)]))
+    device = [(kv.to(DEV), on(DEV, s.astype(np.int32))[0]) for kv, s in zip(kvs, slot_maps)]
+    torch.cuda.synchronize()
+    for kv, slots in device:
+        op.cache_append(kv, cache, slots)
+    for kv, slots in zip(kvs, slot_maps):
+        want_v, want_s = append_ref(kv.double().numpy(), want_v, want_s, slots)
+    assert np.array_equal(cache.scales.cpu().numpy(), want_s) and np.array_equal(cache.values.float().cpu().numpy(), want_v)

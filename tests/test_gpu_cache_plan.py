@@ -106,3 +106,26 @@ def test_on_another_stream_and_in_a_graph():
         torch.cuda.synchronize()
         want = plan_ref(lens, new_len, table, stack, free, 32, 160, 9)
         assert np.array_equal(p.slots.cpu().numpy(), want.slots) and np.array_equal(p.query_meta.cpu().numpy(), want.query_meta)
+
+
+def test_steps_queued_one_behind_the_other():
+    # each plan takes what the one before left, with nothing between the calls
+    from test_operator_b200 import op
+    n, page, calls, rows = 700, 16, 20, 800
+    rng = np.random.default_rng(8)
+    table, n_pages = np.full((n, 4), -1, dtype=np.int32), 1500
+    stack = rng.permutation(n_pages).astype(np.int32)
+    news = [np.where(rng.random(n) < 0.1, -1, 1).astype(np.int32) for _ in range(calls)]
+    d_table, d_stack, d_len, d_count = on(DEV, table, stack, np.zeros(n, dtype=np.int32), np.array([n_pages], dtype=np.int32))
+    d_news = on(DEV, *news)
+    torch.cuda.synchronize()
+    plans = []
+    for new in d_news:
+        plans.append(op.cache_plan(d_len, new, d_table, d_stack, d_count, page, rows, 5))
+        d_len, d_count = plans[-1].kv_len, plans[-1].free_count
+    state = (np.zeros(n, dtype=np.int64), table, stack, n_pages)
+    for new, plan in zip(news, plans):
+        want = plan_ref(state[0], new, state[1], state[2], state[3], page, rows, 5)
+        assert np.array_equal(plan.slots.cpu().numpy(), want.slots) and np.array_equal(plan.kv_len.cpu().numpy(), want.kv_len)
+        state = (want.kv_len, want.block_table, want.free_pages, want.free_count)
+    assert np.array_equal(d_table.cpu().numpy(), state[1]) and np.array_equal(d_stack.cpu().numpy(), state[2])
