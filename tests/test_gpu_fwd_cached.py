@@ -245,3 +245,14 @@ def test_replayed_in_a_graph_beside_another():
     torch.cuda.synchronize()
     for case, (o, lse) in zip(cases, outs):
         _compare(o, lse, attend_ref(*case))
+
+
+@pytest.mark.parametrize("s_q", [2, 150])
+def test_padding_queries_may_hold_anything(s_q):
+    case = _case([700], [s_q], 64, 600, 32, seed=16, pad=40)
+    plain = _run(*case)
+    case[0][s_q:] = float("nan")
+    case[0][s_q + 1::3] = float("inf")
+    o, lse = _run(*case)
+    assert torch.equal(o, plain[0]) and torch.equal(lse, plain[1])
+    assert int(o[s_q:].count_nonzero()) == 0 and bool(lse[s_q:].isposinf().all())
