@@ -112,7 +112,8 @@ def attend_ref(q, values, scales, block_table, indices, query_meta, sm_scale=Non
 
     logits   fp32 sums of 576 products (2 x 576 with q in two parts): 2^-18 of the sum of magnitudes covers their alignment to the largest
              one in every step (probed: 2.5e-6 where one product dominates); q within 2^-9 (both parts rounded) where its row's largest magnitude is 224 to 448.
-    P        half a step of eight significant bits, 2^-8, and half of 2^-9 where the largest P of the row is 64 to 256: 2^-16 of the largest.
+    P        half a step of eight significant bits, 2^-8, and 2^-16 of the largest P of the row (more than the product path takes, 2^-25: the tests of
+             rows with one heavy key have a bound of their own).
     o        half a step of bf16, 2^-8.   ex2, the division and the sums in fp32: a few 2^-22.
     log2 s   is added to the logits and taken out again by way of the sum's logarithm: numbers of size |log2 s|, each of three roundings half of
              2^-23 of it (the logit, the logarithm and its own error), 2^-22 together.

@@ -342,7 +342,8 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int a_mn, i
            (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// The same for kind::f8f6f4 with e4m3 operands (one instruction takes 32 of K).
+// The same for kind::f8f6f4 with e4m3 operands (one instruction takes 32 of K); + kIdescAE5M2: A is e5m2.
+constexpr uint32_t kIdescAE5M2 = 1u << 7;
 __host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N, int a_mn, int b_mn) {
     return (1u << 4) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
            (static_cast<uint32_t>(M >> 4) << 24);

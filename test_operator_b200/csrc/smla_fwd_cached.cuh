@@ -3,15 +3,18 @@
 // Everything that is said at smla_fwd_kernel about the pair of CTAs, the ring, the tensor memory and the work ranges holds here; this is
 // what differs.
 //   operands   kind::f8f6f4 UMMAs on the stored e4m3 numbers as they lie, for K and for V: nothing is converted on the way, and a
-//              gathered row is 576 bytes instead of 1152.  The other side of either product is the sum of two e4m3 numbers, one UMMA each:
-//              q = 2^e (hi + lo) with e from the row's largest magnitude.  A bf16 number has eight significant bits; hi takes four,
+//              gathered row is 576 bytes instead of 1152.  The other side of either product is the sum of two 8-bit numbers, one UMMA each:
+//              q = 2^e (hi + lo), both e4m3, with e from the row's largest magnitude.  A bf16 number has eight significant bits; hi takes four,
 //              lo the other four, so hi + lo is q exactly for what is within 2^-10 of the row's largest, and within 2^-16.8 of the largest
-//              for the rest.  P hi + lo, hi rounded to the nearest: within 2^-9 of P, bf16's is 2^-8, and within half of 2^-9 below 2^-2.
+//              for the rest.  P = hi + lo, hi e4m3 and lo e5m2 (the two terms have instruction descriptors of their own), the heaviest P of a row
+//              between 2^11 and 2^12: within 2^-8 of P, as in bf16, down to 2^-17 of the heaviest, and within 2^-25 of the heaviest below.
+//              A row may have one heavy key and thousands of light ones that weigh something together, so the light ones must not be cut off: with lo in
+//              e4m3, whose smallest number is 2^-9, and the heaviest P at 2^6, o lost up to a quarter of itself.  Both forms take the same time.
 //              An 8-bit UMMA takes 32 of K in the time of 16 in bf16, so two of them cost what one contraction in bf16 costs.
 //   scales     of a key's page, s_j.  The logits are x_j = scale 2^e s_j (hi + lo) c_j.  V needs p_j s_j, and that is what is rounded:
 //              P_j = 2^(x_j + log2 s_j - ref), so that the heaviest P_j are alike whatever the pages' scales are: with ref set the
-//              heaviest is 2^6, and ref moves (and O is rescaled) when one comes above 2^8.  The sum is over p_j = P_j / s_j.  A scale is a
-//              power of two: only its exponent is used.
+//              heaviest is 2^11, and ref moves (and O is rescaled) when one comes above 2^12, the most that hi + lo holds.  The sum is over
+//              p_j = P_j / s_j.  A scale is a power of two: only its exponent is used.
 //   lse, o     o = sum P_j c_j / sum p_j, lse = ref + log2 sum p_j; so partial results combine as in bf16.
 //   Q          is split by the softmax warps when the last logits of the query before are there.
 //   producers  look up pages and scales as well, indices two tiles and pages one tile ahead of the gather; softmax reads (s, log2 s, 1 / s) of
@@ -64,7 +67,7 @@ constexpr int kOffMisc = kOffQExp + 2 * 64 * 4;
 constexpr int kMiscBytes = 256;                               // barriers
 constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;      // + alignment slack
 constexpr int kTmemO = 0, kTmemS = 256;
-constexpr float kTop = 6.f, kLag = 2.f;    // log2 of the heaviest P where the reference has just been set, and how much heavier one may come
+constexpr float kTop = 11.f, kLag = 1.f;   // log2 of the heaviest P where the reference has just been set, and how much heavier one may come
 static_assert(kSmemBytes <= 232448, "shared memory of one SM");
 // Steps of 32 keys up to the last slot in use of the iterator's tile; four of them share two slots of V.
 __device__ __forceinline__ int v_steps(const TileIter<1>& it) { return (min(kTileKeys, it.n_cur - it.tile() * kTileKeys) + 31) >> 5; }
@@ -275,7 +278,7 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
                 for (int j = 0; j < kKSlots; ++j) fill(j * 128, j < kKSlots - 1 || uk < 4);
 #pragma unroll
                 for (int i = 0; i < kKeys; ++i) {
-                    // The exponent alone, and not below 2^-100, so that no sum of p = P / s overflows.  The log of a key that takes no part: -inf.
+                    // The exponent alone, and not below 2^-100, so that p = P / s and sums of 2^15 of them do not overflow.  The log of a key that takes no part: -inf.
                     const int e = max((__float_as_int(scale[i]) >> 23 & 0xff) - 127, kMinScaleExp);
                     const uint32_t to = s_base + kOffScale + buffer * (3 * kTileKeys * 4) + (pt + i * kProducerThreads) * 4;
                     st_shared_f32(to, exp2_int(e));
@@ -410,7 +413,7 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
                             for (int kk = 0; kk < 4; ++kk) {   // 32 keys: 32 bytes along P's rows, 32 rows (4 KB) of V
                                 if (kk >= todo) break;
                                 umma_f8_ss_2cta(d, hi | (a + 2 * kk), hi | (bb + kk * (4096 >> 4)), idesc_o, (g >> 1 | kk) != 0 ? 1u : acc0);
-                                umma_f8_ss_2cta(d, hi | (a + (kTerm >> 4) + 2 * kk), hi | (bb + kk * (4096 >> 4)), idesc_o, 1);
+                                umma_f8_ss_2cta(d, hi | (a + (kTerm >> 4) + 2 * kk), hi | (bb + kk * (4096 >> 4)), idesc_o | kIdescAE5M2, 1);
                             }
                             umma_commit_2cta_mask(bar_empty + 8 * s, 3);
                         }
@@ -582,7 +585,7 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
                     x[k] = pack_f32x2(ex2_approx(z.x), ex2_approx(z.y));
                     add = fma_f32x2(x[k], k ? inv.y : inv.x, add);
                 }
-                split_e4m3x4(x[0], x[1], &p_hi[i], &p_lo[i]);
+                split_e4m3_e5m2x4(x[0], x[1], &p_hi[i], &p_lo[i]);
             }
             {
                 const float2 v = unpack_f32x2(add);
