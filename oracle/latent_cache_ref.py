@@ -111,7 +111,7 @@ def attend_ref(q, values, scales, block_table, indices, query_meta, sm_scale=Non
     """In 64 bits, query by query, on q's device, with bounds on what the roundings of the product path can amount to:
 
     logits   fp32 sums of 576 products (2 x 576 with q in two parts): 2^-18 of the sum of magnitudes covers their alignment to the largest
-             one in every step (probed: 2.5e-6 where one product dominates); q within 2^-9 (both parts rounded) where its row's largest magnitude is 224 to 448.
+             one in every step (probed: 2.5e-6 where one product dominates); q within 2^-9 where its row's largest magnitude is 224 to 448 (more than the product path takes, 2^-14).
     P        half a step of eight significant bits, 2^-8, and 2^-16 of the largest P of the row (more than the product path takes, 2^-25: the tests of
              rows with one heavy key have a bound of their own).
     o        half a step of bf16, 2^-8.   ex2, the division and the sums in fp32: a few 2^-22.

@@ -47,34 +47,28 @@ __device__ __forceinline__ __half2 cvt_f16x2_e4m3x2(uint32_t v) {
     return *reinterpret_cast<const __half2*>(&r);
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-// Two numbers of 0 <= x <= 2^12 as the sum of an e4m3 number (hi) and an e5m2 number (lo) each, to eight significant bits from 2^-6 on and to
-// within 2^-14 below.  An e5m2 number is the upper byte of a half.  Below 2^8 hi is x to four bits and lo three bits of what that leaves, at most
-// half of hi's last place.  From 2^8 on hi would not reach: c is x to three bits, hi takes four of what c leaves, and x - hi to three bits is c
-// again.  *lo: halves, whose upper bytes are lo.  (Eleven bits of a half, and its smallest numbers of 2^-24, are more than what is kept.)
-__device__ __forceinline__ uint32_t split_e4m3_e5m2(uint64_t x01, uint32_t* lo) {
+// Two numbers as the sum of an e4m3 number (hi) and an e5m2 number (lo) each: hi is x to four significant bits and lo three bits of what that
+// leaves, at most half of hi's last place.  For |x| <= 448: to eight bits from 2^-6 on, exactly where x has no more than eight, and to within 2^-14
+// below.  With kLarge for 0 <= x <= 2^12: from 2^8 on, where hi would not reach, c is x to three bits, hi takes four of what c leaves, and x - hi to
+// three bits is c again.  An e5m2 number is the upper byte of a half; *lo: halves, whose upper bytes are lo.  (Eleven bits of a half, and its
+// smallest numbers of 2^-24, are more than what is kept.)
+template <bool kLarge> __device__ __forceinline__ uint32_t split_e4m3_e5m2(uint64_t x01, uint32_t* lo) {
     const float2 a = unpack_f32x2(x01);
     const __half2 x = __floats2half2_rn(a.x, a.y);
-    const uint32_t c = (half2_bits(x) + 0x00800080u) & 0xff00ff00u & __hge2_mask(x, __floats2half2_rn(256.f, 256.f));
-    const uint32_t hi = cvt_e4m3x2_f16x2(__hsub2(x, *reinterpret_cast<const __half2*>(&c)));
+    __half2 main = x;
+    if constexpr (kLarge) {
+        const uint32_t c = (half2_bits(x) + 0x00800080u) & 0xff00ff00u & __hge2_mask(x, __floats2half2_rn(256.f, 256.f));
+        main = __hsub2(x, *reinterpret_cast<const __half2*>(&c));
+    }
+    const uint32_t hi = cvt_e4m3x2_f16x2(main);
     *lo = half2_bits(__hsub2(x, cvt_f16x2_e4m3x2(hi))) + 0x00800080u;
     return hi;
 }
-__device__ __forceinline__ void split_e4m3_e5m2x4(uint64_t x01, uint64_t x23, uint32_t* hi, uint32_t* lo) {
+template <bool kLarge> __device__ __forceinline__ void split_e4m3_e5m2x4(uint64_t x01, uint64_t x23, uint32_t* hi, uint32_t* lo) {
     uint32_t l01, l23;
-    const uint32_t h01 = split_e4m3_e5m2(x01, &l01), h23 = split_e4m3_e5m2(x23, &l23);
+    const uint32_t h01 = split_e4m3_e5m2<kLarge>(x01, &l01), h23 = split_e4m3_e5m2<kLarge>(x23, &l23);
     *hi = h01 | h23 << 16;
     *lo = __byte_perm(l01, l23, 0x7531);
-}
-// Four numbers as the sum of two e4m3 numbers each, hi cut off after four significant bits: exact for numbers of eight bits from 2^-2 on, within half of 2^-9
-// from 2^-6 on, within 2^-9 below (there hi is rounded too).
-__device__ __forceinline__ void split_cut_e4m3x4(uint64_t x01, uint64_t x23, uint32_t* hi, uint32_t* lo) {
-    const float2 a = unpack_f32x2(x01), b = unpack_f32x2(x23);
-    auto cut = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xfff00000u); };
-    const float2 c = make_float2(cut(a.x), cut(a.y)), d = make_float2(cut(b.x), cut(b.y));
-    *hi = cvt_e4m3x4(c.x, c.y, d.x, d.y);
-    const uint64_t minus = pack_f32x2(-1.f, -1.f);
-    const float2 e = unpack_f32x2(fma_f32x2(pack_f32x2(c.x, c.y), minus, x01)), f = unpack_f32x2(fma_f32x2(pack_f32x2(d.x, d.y), minus, x23));
-    *lo = cvt_e4m3x4(e.x, e.y, f.x, f.y);
 }
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
     uint32_t h;

@@ -3,13 +3,14 @@
 // Everything that is said at smla_fwd_kernel about the pair of CTAs, the ring, the tensor memory and the work ranges holds here; this is
 // what differs.
 //   operands   kind::f8f6f4 UMMAs on the stored e4m3 numbers as they lie, for K and for V: nothing is converted on the way, and a
-//              gathered row is 576 bytes instead of 1152.  The other side of either product is the sum of two 8-bit numbers, one UMMA each:
-//              q = 2^e (hi + lo), both e4m3, with e from the row's largest magnitude.  A bf16 number has eight significant bits; hi takes four,
-//              lo the other four, so hi + lo is q exactly for what is within 2^-10 of the row's largest, and within 2^-16.8 of the largest
-//              for the rest.  P = hi + lo, hi e4m3 and lo e5m2 (the two terms have instruction descriptors of their own), the heaviest P of a row
-//              between 2^11 and 2^12: within 2^-8 of P, as in bf16, down to 2^-17 of the heaviest, and within 2^-25 of the heaviest below.
-//              A row may have one heavy key and thousands of light ones that weigh something together, so the light ones must not be cut off: with lo in
-//              e4m3, whose smallest number is 2^-9, and the heaviest P at 2^6, o lost up to a quarter of itself.  Both forms take the same time.
+//              gathered row is 576 bytes instead of 1152.  The other side of either product is the sum of an e4m3 (hi) and an e5m2 number (lo), a UMMA
+//              each, with instruction descriptors of their own: q = 2^e (hi + lo) with e from the row's largest magnitude.  A bf16 number has eight
+//              significant bits; hi to the nearest leaves a whole number of at most eight of the last place, which the three bits of lo hold.
+//              So hi + lo is q exactly for what is within 2^-13 of the row's largest, and within 2^-21 of the largest for the rest.
+//              P = hi + lo with the heaviest P of a row between 2^11 and 2^12: within 2^-8 of P, as in bf16, down to 2^-17 of the heaviest, and
+//              within 2^-25 of the heaviest below.  A row may have one heavy key and thousands of light ones that weigh something together, so the
+//              light ones must not be cut off: with lo in e4m3, whose smallest number is 2^-9, and the heaviest P at 2^6, o lost up to a quarter of
+//              itself.  Both forms take the same time.
 //              An 8-bit UMMA takes 32 of K in the time of 16 in bf16, so two of them cost what one contraction in bf16 costs.
 //   scales     of a key's page, s_j.  The logits are x_j = scale 2^e s_j (hi + lo) c_j.  V needs p_j s_j, and that is what is rounded:
 //              P_j = 2^(x_j + log2 s_j - ref), so that the heaviest P_j are alike whatever the pages' scales are: with ref set the
@@ -103,8 +104,8 @@ __device__ __noinline__ void split_row(const __nv_bfloat16* row, uint32_t image,
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = mul_f32x2(pack_f32x2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)), f2);
         uint32_t h[2], l[2];
-        split_cut_e4m3x4(x[0], x[1], &h[0], &l[0]);
-        split_cut_e4m3x4(x[2], x[3], &h[1], &l[1]);
+        split_e4m3_e5m2x4<false>(x[0], x[1], &h[0], &l[0]);
+        split_e4m3_e5m2x4<false>(x[2], x[3], &h[1], &l[1]);
         const int unit = (j & 1) * 4 + (u >> 1);
         const uint32_t to_hi = to + (j >> 1) * 2 * kTerm + ((unit ^ (r & 7)) << 4);
         const uint32_t to_lo = j < 8 ? to_hi + kTerm : to + 8 * kTerm + (((4 + unit) ^ (r & 7)) << 4);
@@ -385,7 +386,7 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
                             for (int kk = 0; kk < 4; ++kk) {
                                 if (kk >= 2 && !whole) break;
                                 umma_f8_ss_2cta(d, hi | (a + 2 * kk), hi | (bb + 2 * kk), idesc_s, (j | kk) != 0);
-                                umma_f8_ss_2cta(d, hi | (a + to_lo + 2 * kk), hi | (bb + 2 * kk), idesc_s, 1);
+                                umma_f8_ss_2cta(d, hi | (a + to_lo + 2 * kk), hi | (bb + 2 * kk), idesc_s | kIdescAE5M2, 1);
                             }
                             umma_commit_2cta_mask(bar_empty + 8 * s, 3);
                         }
@@ -585,7 +586,7 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
                     x[k] = pack_f32x2(ex2_approx(z.x), ex2_approx(z.y));
                     add = fma_f32x2(x[k], k ? inv.y : inv.x, add);
                 }
-                split_e4m3_e5m2x4(x[0], x[1], &p_hi[i], &p_lo[i]);
+                split_e4m3_e5m2x4<true>(x[0], x[1], &p_hi[i], &p_lo[i]);
             }
             {
                 const float2 v = unpack_f32x2(add);
