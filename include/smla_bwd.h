@@ -212,7 +212,8 @@ int smla_cache_append(const smla_cache_append_params* p, void* workspace, size_t
 /* smla_fwd_run over the cache.  `query_meta` as smla_cache_plan writes it: {request, its tokens in the cache, position for the causal
  * rule, top-k slots in use}; index values are positions in the request, valid in [0, tokens), and with `causal` != 0 only up to the
  * query's position.  A slot whose page number is outside the cache takes no part.  Only a scale's exponent is used, and one below 2^-100
- * counts as 2^-100.  Queries are split into two 8-bit numbers, exactly for what is within 2^-13 of a row's largest magnitude, the rest to within
+ * counts as 2^-100.  The scales of a query's pages may lie up to 2^104 apart (a page of zeros is stored with 2^-100); farther apart, slots in the
+ * pages of the small ones may be left out of the softmax's sum.  Queries are split into two 8-bit numbers, exactly for what is within 2^-13 of a row's largest magnitude, the rest to within
  * 2^-21 of that; a row of q that holds an infinity gives NaN.  What is rounded on the way to o is a slot's weight times the scale of its page:
  * to eight significant bits, as in bf16, down to 2^-17 of the largest one of the (query, head), and to within 2^-25 of that below. */
 typedef struct smla_fwd_cached_params {

@@ -17,10 +17,10 @@ namespace smla {
 constexpr int kMinScaleExp = -100;          // rows are stored with a scale of 2^-100 at least
 constexpr int kMaxPageRows = 128;
 
-// The smallest e >= kMinScaleExp with amax <= 448 * 2^e (448: the largest e4m3 number, 1.75 * 2^8), for a finite amax >= 0.
-__device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
+// The smallest e >= min_exp with amax <= 448 * 2^e (448: the largest e4m3 number, 1.75 * 2^8), for a finite amax >= 0.
+__device__ __forceinline__ int scale_exp(uint32_t amax_bits, int min_exp) {
     const int e = static_cast<int>(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return max(e, kMinScaleExp);
+    return max(e, min_exp);
 }
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
@@ -358,7 +358,7 @@ __device__ __forceinline__ void append_write_page(const CacheAppendArgs& a, int 
         for (int i = slot; i < n; i += kAppendSide) top = finite_max_bf16x2(top, source(i));
         top = append_block_max(top, sh);
     }
-    const float wanted = exp2_int(scale_exp(top << 16));
+    const float wanted = exp2_int(scale_exp(top << 16, kMinScaleExp));
     const bool anew = sh.win[0] >= 0;             // its first row is written: what it held belongs to nobody
     const float scale = anew ? wanted : fmaxf(old, wanted);
     uint8_t* base = a.values + static_cast<size_t>(page) * page_rows * kDQK;
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kAppendThreads, 6) smla_cache_append_listed_ke
             finite = max(max(finites[0], finites[1]), max(finites[2], finites[3]));
             parity ^= 1;                          // (the next page's sync comes before this place is written again)
             const bool anew = sh.win[0] >= 0;
-            const float wanted = exp2_int(scale_exp(finite << 16)), scale = anew ? wanted : fmaxf(old, wanted);
+            const float wanted = exp2_int(scale_exp(finite << 16, kMinScaleExp)), scale = anew ? wanted : fmaxf(old, wanted);
             uint8_t* base = a.values + static_cast<size_t>(mine.x) * page_rows * kDQK;
             if (!anew && scale > old) append_rescale(sh, base, r0, r1, old / scale);
             if (threadIdx.x == 0 && rank == 0) a.scales[mine.x] = scale;

@@ -70,6 +70,7 @@ constexpr int kSmemBytes = kOffMisc + kMiscBytes + 1024;      // + alignment sla
 constexpr int kTmemO = 0, kTmemS = 256;
 constexpr float kTop = 11.f, kLag = 1.f;   // log2 of the heaviest P where the reference has just been set, and how much heavier one may come
 static_assert(kSmemBytes <= 232448, "shared memory of one SM");
+constexpr int kMinQExp = -126;             // smallest 2^e of a row of Q, the smallest normal number (its inverse is one too)
 // Steps of 32 keys up to the last slot in use of the iterator's tile; four of them share two slots of V.
 __device__ __forceinline__ int v_steps(const TileIter<1>& it) { return (min(kTileKeys, it.n_cur - it.tile() * kTileKeys) + 31) >> 5; }
 __device__ __forceinline__ int v_slots(int steps) { return 2 * ((steps + 3) >> 2); }
@@ -92,7 +93,7 @@ __device__ __noinline__ void split_row(const __nv_bfloat16* row, uint32_t image,
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const bool bad = top >= 0x7f800000u;
-    const int e = bad ? 0 : scale_exp(top);
+    const int e = bad ? 0 : scale_exp(top, kMinQExp);
     const float f = bad ? __int_as_float(0x7fffffff) : exp2_int(-e);
     if (u == 0) st_shared_f32(exps + r * 4, exp2_int(e));
     const uint64_t f2 = pack_f32x2(f, f);
@@ -536,14 +537,14 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
             __syncwarp();
             // the S buffer has been read (tcgen05.wait::ld), which is all the issuer needs to know
             if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + 8 * b);
-            // x + log2 s
+            // x + log2 s.  (The scales of q and of the page first: a large one of the page alone would take the products beyond fp32.)
             const uint64_t q2 = pack_f32x2(q_scale, q_scale);
             uint64_t y[16];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const ulonglong2 s4 = ld_shared_f32x4(scale_s + 16 * i), l4 = ld_shared_f32x4(scale_s + kTileKeys * 4 + 16 * i);
-                y[2 * i] = fma_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sv[4 * i]), __uint_as_float(sv[4 * i + 1])), s4.x), q2, l4.x);
-                y[2 * i + 1] = fma_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sv[4 * i + 2]), __uint_as_float(sv[4 * i + 3])), s4.y), q2, l4.y);
+                y[2 * i] = fma_f32x2(pack_f32x2(__uint_as_float(sv[4 * i]), __uint_as_float(sv[4 * i + 1])), mul_f32x2(s4.x, q2), l4.x);
+                y[2 * i + 1] = fma_f32x2(pack_f32x2(__uint_as_float(sv[4 * i + 2]), __uint_as_float(sv[4 * i + 3])), mul_f32x2(s4.y, q2), l4.y);
             }
             if (mask != 0xffffffffu) {                       // warp-uniform
 #pragma unroll

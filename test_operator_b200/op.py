@@ -856,7 +856,7 @@ def mla_fwd_cached(q: torch.Tensor, cache: LatentCache, block_table: torch.Tenso
     query's own request; `query_meta` [s_q, 4] is what `cache_plan` makes: request, its tokens in the cache, the query's position, top-k slots
     in use (all int32).  A slot counts if it is in use, its position lies in the request's tokens and, with `causal`, not behind the query's,
     and its page is one of the cache.  A query without such a slot (a padding row) gives o = 0 and lse = +inf.  Of a page's scale the exponent
-    is used.  A slot's weight times its page's scale is rounded to eight significant bits, as in bf16, down to 2^-17 of the largest one of
+    is used, and those of a query's pages may lie up to 2^104 apart.  A slot's weight times its page's scale is rounded to eight significant bits, as in bf16, down to 2^-17 of the largest one of
     the (query, head), and to within 2^-25 of that below.  Prompts and single tokens take the same call."""
     if workspace is None and not (workspace_budget or check_device_status):
         out = _host().fwd_cached(q, cache, block_table, indices, query_meta, sm_scale, 1 if causal else 0, 1 if lse_is_base2 else 0)
