@@ -191,6 +191,12 @@ typedef struct smla_cache_plan_params {
     int32_t n_requests, max_pages, n_free, page_size, max_tokens, topk;
 } smla_cache_plan_params;
 int smla_cache_plan(const smla_cache_plan_params* p, void* stream);
+/* The same where tokens are dropped first (draft tokens that were not accepted): the last rejected[i] of the kv_len[i] tokens of request i, which
+ * goes on behind the others in the pages it has.  Those that it does not need after the step go back onto the stack, before new ones
+ * are taken (in order of requests and pages, as those of requests that end).  `rejected` i32 [n_requests] or null; below 0 counts as 0, and no
+ * more than kv_len is dropped; a request that is not admitted keeps the dropped tokens too (kv_len as it was), for the next step to drop.  Setting kv_len back
+ * by hand instead would lose the pages behind it: a request's pages are those of kv_len tokens. */
+int smla_cache_plan_rejecting(const smla_cache_plan_params* p, const int32_t* rejected, void* stream);
 
 /* Writes rows into the cache.  kv: bf16 [n_rows, 576] with kv_stride elements from row to row (a multiple of 8), slots i32 [n_rows]; rows
  * whose slot is outside the cache are left out, of several rows with one slot the last one is kept.  A page whose row 0 is among the

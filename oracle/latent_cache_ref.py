@@ -26,16 +26,19 @@ class Plan(NamedTuple):
     free_pages: np.ndarray
 
 
-def plan_ref(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk) -> Plan:
+def plan_ref(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk, rejected=None) -> Plan:
     table, free = np.array(block_table), np.array(free_pages)
     kv_len, new_len = [int(v) for v in kv_len], [int(v) for v in new_len]
     stack = [int(v) for v in free[:free_count]]
     n = len(kv_len)
     room = table.shape[1] * page_size
     pages = lambda tokens: -(-tokens // page_size)  # noqa: E731
+    keep = [k - min(max(int(r), 0), max(k, 0)) for k, r in zip(kv_len, [0] * n if rejected is None else rejected)]
+    row_end = np.cumsum([max(m, 0) for m in new_len])
+    fits = lambda i: new_len[i] >= 0 and 0 <= kv_len[i] <= room and keep[i] + new_len[i] <= room and row_end[i] <= max_tokens  # noqa: E731
     for i in range(n):
-        if new_len[i] < 0:
-            for k in range(pages(min(max(kv_len[i], 0), room))):
+        if new_len[i] < 0 or fits(i):          # all pages of a request that ends, those behind the last token of one that goes on
+            for k in range(0 if new_len[i] < 0 else pages(keep[i] + new_len[i]), pages(min(max(kv_len[i], 0), room))):
                 stack.append(int(table[i, k]))
                 if len(stack) <= len(free):
                     free[len(stack) - 1] = table[i, k]
@@ -48,17 +51,17 @@ def plan_ref(kv_len, new_len, block_table, free_pages, free_count, page_size, ma
             after[i] = 0
             continue
         row0, first = first, first + new_len[i]
-        if kv_len[i] < 0 or kv_len[i] + new_len[i] > room or first > max_tokens:
+        if not fits(i):
             continue
-        have, want = pages(kv_len[i]), pages(kv_len[i] + new_len[i])
+        have, want = pages(kv_len[i]), pages(keep[i] + new_len[i])
         if want > have and (short or want - have > len(stack)):
             short = True
             continue
         for k in range(have, want):
             table[i, k] = stack.pop()
-        after[i], admitted[i] = kv_len[i] + new_len[i], new_len[i]
+        after[i], admitted[i] = keep[i] + new_len[i], new_len[i]
         for j in range(new_len[i]):
-            pos = kv_len[i] + j
+            pos = keep[i] + j
             slots[row0 + j] = table[i, pos // page_size] * page_size + pos % page_size
             meta[row0 + j] = (i, after[i], pos, topk)
     return Plan(slots, meta, np.array(after), min(len(stack), len(free)), np.array(admitted), table, free)

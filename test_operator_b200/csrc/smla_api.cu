@@ -942,7 +942,9 @@ int smla_fwd_cached_run(const smla_fwd_cached_params* p, void* workspace, size_t
     return pl.h_pad == 64 ? launch_fwd_cached_chain<64>(p, &f, pl, ws, st) : launch_fwd_cached_chain<128>(p, &f, pl, ws, st);
 }
 
-int smla_cache_plan(const smla_cache_plan_params* p, void* stream) {
+int smla_cache_plan(const smla_cache_plan_params* p, void* stream) { return smla_cache_plan_rejecting(p, nullptr, stream); }
+
+int smla_cache_plan_rejecting(const smla_cache_plan_params* p, const int32_t* rejected, void* stream) {
     using namespace smla;
     g_last_launches = 0;
     if (!p || !p->kv_len || !p->new_len || !p->free_count || !p->block_table || !p->free_pages || !p->kv_len_out || !p->free_count_out || !p->admitted)
@@ -956,11 +958,16 @@ int smla_cache_plan(const smla_cache_plan_params* p, void* stream) {
         return SMLA_ERR_BAD_ARG;
     const int smem = (4 * p->n_requests + 3) * 4;
     static std::atomic<bool> attr_done[kMaxDevices];
-    if (!once_per_device(attr_done, [] { return set_smem(smla_cache_plan_kernel, (4 * kMaxCacheRequests + 3) * 4); })) return SMLA_ERR_LAUNCH;
+    const auto set = [] {
+        constexpr int most = (4 * kMaxCacheRequests + 3) * 4;
+        return set_smem(smla_cache_plan_kernel<false>, most) && set_smem(smla_cache_plan_kernel<true>, most);
+    };
+    if (!once_per_device(attr_done, set)) return SMLA_ERR_LAUNCH;
     CachePlanArgs a{};
     a.kv_len = p->kv_len;
     a.new_len = p->new_len;
     a.free_count = p->free_count;
+    a.rejected = rejected;
     a.table = p->block_table;
     a.free_pages = p->free_pages;
     a.slots = p->slots;
@@ -979,7 +986,7 @@ int smla_cache_plan(const smla_cache_plan_params* p, void* stream) {
     const long long by_tokens = (p->max_tokens + kCachePlanThreads - 1) / kCachePlanThreads;
     const long long by_pages = static_cast<long long>(p->n_requests) * p->max_pages / (8 * kCachePlanThreads);
     const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>(kSmCount, std::max(by_tokens, by_pages))));
-    launch(smla_cache_plan_kernel, blocks, kCachePlanThreads, smem, reinterpret_cast<cudaStream_t>(stream), true, 1, a);
+    launch(rejected ? smla_cache_plan_kernel<true> : smla_cache_plan_kernel<false>, blocks, kCachePlanThreads, smem, reinterpret_cast<cudaStream_t>(stream), true, 1, a);
     return cudaGetLastError() == cudaSuccess ? SMLA_OK : SMLA_ERR_LAUNCH;
 }
 

@@ -83,10 +83,13 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
 // of the pages that change hands, so one launch does it, with no prefix sums in memory.  That needs no order between the blocks: what is
 // read (free_pages below free_count, the block table's entries of pages that requests had before the call) is not written by any
 // of them.  A page that is given back and taken again in the same call is looked up in the row of the request that gives it.
+// A request whose last tokens are dropped keeps its pages and writes its new tokens over them; what it does not need any more it gives back, and then it
+// takes none.
 // Bound by latency: a launch, two dependent loads and three block sums.
 // =============================================================================================
 struct CachePlanArgs {
     const int *kv_len, *new_len, *free_count;
+    const int* rejected;          // (kRejects)
     int *table, *free_pages;
     int *slots, *kv_len_out, *free_count_out, *admitted;
     int4* meta;
@@ -127,11 +130,11 @@ __device__ __forceinline__ int block_exclusive_capped_sum(int v, int cap, int* w
     return lane ? min(before + left, cap) : before;
 }
 
-__global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(const CachePlanArgs a) {
+template <bool kRejects> __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(const CachePlanArgs a) {
     extern __shared__ int plan_smem[];
     __shared__ int warp_sums[kCachePlanThreads / 32];
     int* first = plan_smem;                       // [n_req + 1] tokens of the requests before, at most max_tokens + 1
-    int* len = first + a.n_req + 1;               // [n_req] kv_len, ~kv_len of a request that gets no row
+    int* len = first + a.n_req + 1;               // [n_req] tokens that stay, ~ of them for a request that gets no row
     int* needx = len + a.n_req;                   // [n_req + 1] new pages asked for by the requests before
     int* backx = needx + a.n_req + 1;             // [n_req + 1] pages given back by the requests before
     pdl_wait();
@@ -143,32 +146,36 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
     const int room = a.max_pages << a.page_shift;                      // (below 2^31: checked on the host)
     auto length = [&](int i) { return min(max(__ldg(a.kv_len + i), 0), room); };
     auto pages_of = [&](int tokens) { return (tokens + page - 1) >> a.page_shift; };
-    int back = 0, tokens = 0;
-    for (int i = i0; i < i1; ++i) {
-        const int n = __ldg(a.new_len + i);
-        if (n < 0) back += pages_of(length(i));
-        else tokens = min(tokens + min(n, cap), cap);
-    }
+    auto stays = [&](int i, int old) { return kRejects ? old - min(max(__ldg(a.rejected + i), 0), max(old, 0)) : old; };
+    int tokens = 0;
+    for (int i = i0; i < i1; ++i) tokens = min(tokens + min(max(__ldg(a.new_len + i), 0), cap), cap);
     int n_back, n_tokens, n_need, n_taken;
-    const int back0 = block_exclusive_sum(back, warp_sums, &n_back);
     const int first0 = block_exclusive_capped_sum(tokens, cap, warp_sums, &n_tokens);
-    // what request i asks for, given the tokens before it; -1: it cannot have its rows whatever is free
-    auto need_of = [&](int i, int n, int before) {
-        const int old = __ldg(a.kv_len + i);
-        if (n < 0 || old < 0 || old > room || n > room - old || before + min(n, cap) > a.max_tokens) return -1;
-        return pages_of(old + n) - pages_of(old);
+    // what request i asks for beyond the pages it has, given the tokens before it; -1: it cannot have its rows whatever is free.  *give: pages that
+    // it gives back
+    auto need_of = [&](int i, int n, int before, int* give) {
+        const int old = __ldg(a.kv_len + i), keep = stays(i, old);
+        *give = n < 0 ? pages_of(length(i)) : 0;
+        if (n < 0 || old < 0 || old > room || n > room - keep || before + min(n, cap) > a.max_tokens) return -1;
+        const int more = pages_of(keep + n) - pages_of(old);
+        *give = max(-more, 0);
+        return max(more, 0);
     };
-    int need = 0;
+    int need = 0, back = 0;
     for (int i = i0, f = first0; i < i1; ++i) {
         const int n = __ldg(a.new_len + i);
-        need += max(need_of(i, n, f), 0);
+        int give;
+        need += max(need_of(i, n, f, &give), 0);
+        back += give;
         f = min(f + min(max(n, 0), cap), cap);
     }
     const int need0 = block_exclusive_sum(need, warp_sums, &n_need);
+    const int back0 = block_exclusive_sum(back, warp_sums, &n_back);
     const int stack = n_free + n_back;
     int taken = 0;
     for (int i = i0, f = first0, u = need0, b = back0; i < i1; ++i) {
-        const int n = __ldg(a.new_len + i), old = length(i), want = need_of(i, n, f);
+        int give;
+        const int n = __ldg(a.new_len + i), old = stays(i, length(i)), want = need_of(i, n, f, &give);
         const bool granted = want >= 0 && (want == 0 || u + want <= stack);
         first[i] = f;
         len[i] = granted ? old : ~old;
@@ -181,17 +188,19 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
         f = min(f + min(max(n, 0), cap), cap);
         u += max(want, 0);
         if (granted) taken += want;
-        if (n < 0) b += pages_of(old);
+        b += give;
     }
     if (threadIdx.x == 0) first[a.n_req] = n_tokens;
     block_exclusive_sum(taken, warp_sums, &n_taken);           // (its barriers: the tables are whole)
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.free_count_out = min(stack - n_taken, a.n_free);
-    // place s of the stack of free pages, the pages given back on top
-    auto stacked = [&](int s) {
-        if (s < n_free) return __ldcg(a.free_pages + s);
-        const int v = s - n_free, i = last_not_above(backx, a.n_req, v);
-        return __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
+    // page v of the ones given back: all of a request that ends, the ones behind its last token of a request that goes on
+    auto given_back = [&](int v) {
+        const int i = last_not_above(backx, a.n_req, v), from = !kRejects || len[i] < 0 ? 0 : pages_of(len[i] + (first[i + 1] - first[i]));
+        return __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + (from + v - backx[i]));
     };
+    // place s of the stack of free pages, the pages given back on top
+    auto stacked = [&](int s) { return s < n_free ? __ldcg(a.free_pages + s) : given_back(s - n_free); };
+    auto pages_held = [&](int i) { return pages_of(kRejects ? length(i) : len[i]); };      // by a request that gets its rows
     const int at = blockIdx.x * kCachePlanThreads + threadIdx.x, step = gridDim.x * kCachePlanThreads;
     for (int t = at; t < a.max_tokens; t += step) {
         int slot = -1;
@@ -199,7 +208,7 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
         if (t < n_tokens) {
             const int i = last_not_above(first, a.n_req, t), old = len[i];
             if (old >= 0) {
-                const int pos = old + t - first[i], k = pos >> a.page_shift, have = pages_of(old);
+                const int pos = old + t - first[i], k = pos >> a.page_shift, have = pages_held(i);
                 const int pg = k < have ? __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + k) : stacked(stack - 1 - (needx[i] + k - have));
                 slot = pg * page + (pos & (page - 1));
                 m = make_int4(i, old + (first[i + 1] - first[i]), pos, a.topk);
@@ -210,12 +219,9 @@ __global__ void __launch_bounds__(kCachePlanThreads) smla_cache_plan_kernel(cons
     }
     for (int u = at; u < n_taken; u += step) {
         const int i = last_not_above(needx, a.n_req, u);
-        a.table[static_cast<size_t>(i) * a.max_pages + pages_of(len[i]) + (u - needx[i])] = stacked(stack - 1 - u);
+        a.table[static_cast<size_t>(i) * a.max_pages + pages_held(i) + (u - needx[i])] = stacked(stack - 1 - u);
     }
-    for (int v = at; v < n_back && n_free + v < a.n_free; v += step) {
-        const int i = last_not_above(backx, a.n_req, v);
-        a.free_pages[n_free + v] = __ldcg(a.table + static_cast<size_t>(i) * a.max_pages + (v - backx[i]));
-    }
+    for (int v = at; v < n_back && n_free + v < a.n_free; v += step) a.free_pages[n_free + v] = given_back(v);
 }
 
 // =============================================================================================

@@ -37,7 +37,7 @@ decltype(&smla_fwd_run) g_fwd_run = nullptr;
 decltype(&smla_fwd_workspace_size) g_fwd_size = nullptr;
 decltype(&smla_bwd_run_stages) g_bwd_run = nullptr;
 decltype(&smla_bwd_workspace_size) g_bwd_size = nullptr;
-decltype(&smla_cache_plan) g_cache_plan = nullptr;
+decltype(&smla_cache_plan_rejecting) g_cache_plan = nullptr;
 decltype(&smla_cache_append) g_cache_append = nullptr;
 decltype(&smla_cache_append_workspace_size) g_append_size = nullptr;
 decltype(&smla_fwd_cached_run) g_cached_run = nullptr;
@@ -218,12 +218,12 @@ at::Tensor part_of(const at::Tensor& buffer, int64_t begin, at::IntArrayRef size
     return t;
 }
 
-// cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk) -> (slots, query_meta, kv_len, free_count,
-// admitted), a status, or None.
+// cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk[, rejected or None]) -> (slots, query_meta, kv_len,
+// free_count, admitted), a status, or None.
 PyObject* cache_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     smla_cache_plan_params p{};
-    if (n != 8 || !g_cache_plan || !int32_of(a[5], &p.page_size) || !int32_of(a[6], &p.max_tokens) || !int32_of(a[7], &p.topk)) Py_RETURN_NONE;
+    if (n < 8 || n > 9 || !g_cache_plan || !int32_of(a[5], &p.page_size) || !int32_of(a[6], &p.max_tokens) || !int32_of(a[7], &p.topk)) Py_RETURN_NONE;
     const at::Tensor* t[5];
     for (int i = 0; i < 5; ++i)
         if (!(t[i] = plain(a[i], at::kInt)) || t[i]->get_device() != t[0]->get_device() || t[i]->dim() != (i == 2 ? 2 : 1)) Py_RETURN_NONE;
@@ -231,6 +231,12 @@ PyObject* cache_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (t[1]->size(0) != requests || t[2]->size(0) != requests || t[4]->size(0) != 1 || requests > 8192 || t[2]->size(1) > INT32_MAX ||
         t[3]->size(0) > INT32_MAX || p.max_tokens <= 0 || p.max_tokens >= 1 << 30)
         Py_RETURN_NONE;
+    const int32_t* rejected = nullptr;
+    if (n == 9 && a[8] != Py_None) {
+        const at::Tensor* r = plain(a[8], at::kInt);
+        if (!r || r->get_device() != t[0]->get_device() || r->dim() != 1 || r->size(0) != requests) Py_RETURN_NONE;
+        rejected = static_cast<const int32_t*>(r->data_ptr());
+    }
     const c10::cuda::CUDAGuard guard(t[0]->device());
     // one allocation: query_meta (16-byte aligned), slots, kv_len, admitted, free_count
     const int64_t T = p.max_tokens;
@@ -252,7 +258,7 @@ PyObject* cache_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(t[0]->get_device()).stream();
     int st;
     Py_BEGIN_ALLOW_THREADS
-    st = g_cache_plan(&p, stream);
+    st = g_cache_plan(&p, rejected, stream);
     Py_END_ALLOW_THREADS
     if (st != SMLA_OK) return PyLong_FromLong(st);
     const at::Tensor parts[5] = {part_of(buffer, 4 * T, {T}), part_of(buffer, 0, {T, 4}), part_of(buffer, 5 * T, {requests}),
@@ -448,7 +454,7 @@ PyObject* delta_wait(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// init(addresses of smla_fwd_run, smla_fwd_workspace_size, smla_bwd_run_stages, smla_bwd_workspace_size, smla_cache_plan, smla_cache_append,
+// init(addresses of smla_fwd_run, smla_fwd_workspace_size, smla_bwd_run_stages, smla_bwd_workspace_size, smla_cache_plan_rejecting, smla_cache_append,
 // smla_cache_append_workspace_size, smla_fwd_cached_run, smla_fwd_cached_workspace_size)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* f[9];

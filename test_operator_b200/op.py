@@ -149,6 +149,8 @@ def load_library() -> ctypes.CDLL:
         lib.smla_fwd_run.argtypes = [ctypes.POINTER(_FwdParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.smla_cache_plan.restype = ctypes.c_int
         lib.smla_cache_plan.argtypes = [ctypes.POINTER(_CachePlanParams), ctypes.c_void_p]
+        lib.smla_cache_plan_rejecting.restype = ctypes.c_int
+        lib.smla_cache_plan_rejecting.argtypes = [ctypes.POINTER(_CachePlanParams), ctypes.c_void_p, ctypes.c_void_p]
         lib.smla_cache_append_workspace_size.restype = ctypes.c_size_t
         lib.smla_cache_append_workspace_size.argtypes = [ctypes.c_int32]
         lib.smla_cache_append.restype = ctypes.c_int
@@ -253,7 +255,7 @@ def _load_host(lib):
         module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_smla_host", loader, origin=path))
         loader.exec_module(module)
         module.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in
-                      (lib.smla_fwd_run, lib.smla_fwd_workspace_size, lib.smla_bwd_run_stages, lib.smla_bwd_workspace_size, lib.smla_cache_plan,
+                      (lib.smla_fwd_run, lib.smla_fwd_workspace_size, lib.smla_bwd_run_stages, lib.smla_bwd_workspace_size, lib.smla_cache_plan_rejecting,
                        lib.smla_cache_append, lib.smla_cache_append_workspace_size, lib.smla_fwd_cached_run, lib.smla_fwd_cached_workspace_size)))
         return module
     except Exception as e:
@@ -770,7 +772,7 @@ def _check_cache(cache, device) -> None:
 
 
 def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
-               page_size: int, max_tokens: int, topk: int) -> CachePlan:
+               page_size: int, max_tokens: int, topk: int, rejected: Optional[torch.Tensor] = None) -> CachePlan:
     """Tables of one serving step, made on the GPU from the requests' lengths: pages for the new tokens, the slot of each of them, and the
     query table of `mla_fwd_cached`.  All tensors int32 on one device.
 
@@ -780,8 +782,13 @@ def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.T
     successors.  Token rows are packed in order of requests, new_len[i] of each; rows behind the last of them, up to max_tokens (a fixed
     size for a step that is captured in a graph), have slot -1 and an empty query.  Requests are served in order; one for which the pages, the
     table's width or the rows do not suffice gets nothing in this step (`admitted` 0, its rows' slots -1), nor does a later one that needs a
-    page once there were too few.  At most 8192 requests; nothing synchronises."""
-    out = _host().cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk)
+    page once there were too few.  At most 8192 requests; nothing synchronises.
+
+    rejected [n_requests], where draft tokens were not accepted: the last rejected[i] of the kv_len[i] tokens are dropped before the step; the request goes
+    on behind the others in the pages it has, and those that it does not need after the step go back onto the stack.  (kv_len set back by hand would
+    lose them: a request's pages are those of kv_len tokens.)  A request that gets nothing in this step keeps the dropped tokens too, for the next
+    step to drop."""
+    out = _host().cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk, rejected)
     if type(out) is tuple:
         return CachePlan._make(out)
     _check(isinstance(kv_len, torch.Tensor) and kv_len.is_cuda, "kv_len must be a CUDA tensor")
@@ -793,6 +800,8 @@ def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.T
     _check_int32(block_table, (n, None), device, "block_table")
     _check_int32(free_pages, (None,), device, "free_pages")
     _check_int32(free_count, (1,), device, "free_count")
+    if rejected is not None:
+        _check_int32(rejected, (n,), device, "rejected")
     _check(page_size in _PAGE_SIZES, f"page_size must be one of {_PAGE_SIZES}, got {page_size}")
     _check(0 <= max_tokens < 2 ** 30 and 0 <= topk < 2 ** 31, "max_tokens must be in [0, 2^30), topk in [0, 2^31)")
     _check(block_table.shape[1] > 0 and free_pages.shape[0] > 0, "block_table and free_pages must not be empty")
@@ -806,7 +815,8 @@ def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.T
         p = _CachePlanParams(kv_len.data_ptr(), new_len.data_ptr(), free_count.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
                              plan.slots.data_ptr(), plan.query_meta.data_ptr(), plan.kv_len.data_ptr(), plan.free_count.data_ptr(),
                              plan.admitted.data_ptr(), n, block_table.shape[1], free_pages.shape[0], page_size, max_tokens, topk)
-        _raise_status(lib, lib.smla_cache_plan(ctypes.byref(p), _raw_stream(index)), "smla_cache_plan")
+        st = lib.smla_cache_plan_rejecting(ctypes.byref(p), rejected.data_ptr() if rejected is not None else None, _raw_stream(index))
+        _raise_status(lib, st, "smla_cache_plan")
     return plan
 
 
