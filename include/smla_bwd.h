@@ -195,7 +195,8 @@ int smla_cache_plan(const smla_cache_plan_params* p, void* stream);
  * goes on behind the others in the pages it has.  Those that it does not need after the step go back onto the stack, before new ones
  * are taken (in order of requests and pages, as those of requests that end).  `rejected` i32 [n_requests] or null; below 0 counts as 0, and no
  * more than kv_len is dropped; a request that is not admitted keeps the dropped tokens too (kv_len as it was), for the next step to drop.  Setting kv_len back
- * by hand instead would lose the pages behind it: a request's pages are those of kv_len tokens. */
+ * by hand instead would lose the pages behind it: a request's pages are those of kv_len tokens.
+ * Neither call counts a page's holders: a page in the tables of several requests would be given back by each of them. */
 int smla_cache_plan_rejecting(const smla_cache_plan_params* p, const int32_t* rejected, void* stream);
 
 /* Writes rows into the cache.  kv: bf16 [n_rows, 576] with kv_stride elements from row to row (a multiple of 8), slots i32 [n_rows]; rows

@@ -787,7 +787,7 @@ def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.T
     rejected [n_requests], where draft tokens were not accepted: the last rejected[i] of the kv_len[i] tokens are dropped before the step; the request goes
     on behind the others in the pages it has, and those that it does not need after the step go back onto the stack.  (kv_len set back by hand would
     lose them: a request's pages are those of kv_len tokens.)  A request that gets nothing in this step keeps the dropped tokens too, for the next
-    step to drop."""
+    step to drop.  A page must be in the table of one request only: there is no count of holders."""
     out = _host().cache_plan(kv_len, new_len, block_table, free_pages, free_count, page_size, max_tokens, topk, rejected)
     if type(out) is tuple:
         return CachePlan._make(out)
