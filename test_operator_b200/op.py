@@ -760,7 +760,7 @@ def _check_int32(t, shape, device, name) -> None:
            f"{name} must have shape {[('*' if n is None else n) for n in shape]}, got {list(t.shape)}")
 
 
-def _check_cache(cache, device) -> None:
+def _check_cache(cache, device) -> "LatentCache":
     _check(isinstance(cache, tuple) and len(cache) == 2 and all(isinstance(t, torch.Tensor) for t in cache), "cache must be a LatentCache")
     values, scales = cache
     _check(values.is_cuda and scales.is_cuda and values.device == device and scales.device == device, f"the cache must be on {device}")
@@ -769,6 +769,7 @@ def _check_cache(cache, device) -> None:
            f"cache values must be contiguous [n_pages, page_size, {D_QK}] with a page_size of {_PAGE_SIZES}")
     _check(scales.dim() == 1 and scales.shape[0] == values.shape[0] and scales.is_contiguous(), "cache scales must be contiguous [n_pages]")
     _check(values.shape[0] * values.shape[1] < 2 ** 31, "a cache holds less than 2^31 rows")
+    return LatentCache(values, scales)
 
 
 def cache_plan(kv_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
@@ -836,7 +837,7 @@ def cache_append(kv: torch.Tensor, cache: LatentCache, slots: torch.Tensor) -> N
     n = kv.shape[0]
     _check(kv.stride(1) == 1 and (n <= 1 or kv.stride(0) % 8 == 0) and kv.data_ptr() % 16 == 0,
            "kv rows must be contiguous, 16-byte aligned, and a multiple of 8 elements apart")
-    _check_cache(cache, kv.device)
+    cache = _check_cache(cache, kv.device)
     _check_int32(slots, (n,), kv.device, "slots")
     if n == 0:
         return
@@ -882,7 +883,7 @@ def mla_fwd_cached(q: torch.Tensor, cache: LatentCache, block_table: torch.Tenso
     _check(indices.device == q.device, "indices must be on the same device as q")
     topk = indices.shape[-1]
     _check(topk > 0, "topk must be positive")
-    _check_cache(cache, q.device)
+    cache = _check_cache(cache, q.device)
     _check_int32(block_table, (None, None), q.device, "block_table")
     _check_int32(query_meta, (s_q, 4), q.device, "query_meta")
     _check(query_meta.data_ptr() % 16 == 0, "query_meta must be 16-byte aligned")
