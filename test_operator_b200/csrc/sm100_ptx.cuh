@@ -200,8 +200,6 @@ __device__ __forceinline__ bool flag_wait(uint32_t saddr, uint32_t want, const W
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-// (global memory too)
-__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before_sync() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -249,11 +247,6 @@ __device__ __forceinline__ void tma_load_4d_hint(uint32_t dst, const void* tmap,
         "[%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
         ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
         : "memory");
-}
-// Bulk copy of `bytes` (multiple of 16, both addresses 16-byte aligned) from global to this CTA's shared memory, counted on its barrier `bar`.
-__device__ __forceinline__ void bulk_load(uint32_t sdst, const void* gsrc, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sdst), "l"(gsrc), "r"(bytes), "r"(bar)
-                 : "memory");
 }
 // Bulk copy of `bytes` (multiple of 16, both addresses 16-byte aligned) from this CTA's shared memory to global,
 // tracked by the thread's bulk-group; the source may be reused after bulk_wait_read().
