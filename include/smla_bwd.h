@@ -204,6 +204,7 @@ int smla_cache_plan_rejecting(const smla_cache_plan_params* p, const int32_t* re
  * slots starts anew: its scale becomes the smallest power of two (2^-100 at least) that holds the call's rows in the page, and its
  * other rows stay as they are, void.  Any other page's scale grows to that where it is smaller, and the rows it keeps are brought over to the
  * new scale.  Rows are rounded to the nearest; a number that is not finite is stored as a NaN and does not count for the scale.
+ * The time grows with the square of the call's runs (neighbouring rows of one page): long calls are for prompts, whose rows come page by page.
  * `workspace` (256-byte aligned, smla_cache_append_workspace_size() bytes, may be null where that is 0). */
 typedef struct smla_cache_append_params {
     const void* kv;
@@ -220,9 +221,10 @@ int smla_cache_append(const smla_cache_append_params* p, void* workspace, size_t
  * rule, top-k slots in use}; index values are positions in the request, valid in [0, tokens), and with `causal` != 0 only up to the
  * query's position.  A slot whose page number is outside the cache takes no part.  Only a scale's exponent is used, and one below 2^-100
  * counts as 2^-100.  The scales of a query's pages may lie up to 2^104 apart (a page of zeros is stored with 2^-100); farther apart, slots in the
- * pages of the small ones may be left out of the softmax's sum.  Queries are split into two 8-bit numbers, exactly for what is within 2^-13 of a row's largest magnitude, the rest to within
- * 2^-21 of that; a row of q that holds an infinity gives NaN.  What is rounded on the way to o is a slot's weight times the scale of its page:
- * to eight significant bits, as in bf16, down to 2^-17 of the largest one of the (query, head), and to within 2^-25 of that below. */
+ * pages of the small ones may be left out of the softmax's sum.  Queries are split into two 8-bit numbers, exactly for what is within 2^-13 of a
+ * row's largest magnitude, the rest to within 2^-21 of that; a row of q that holds an infinity gives NaN.  What is rounded on the way to o is a
+ * slot's weight times the scale of its page: to eight significant bits, as in bf16, down to 2^-17 of the largest one of the (query, head), and to
+ * within 2^-25 of that below. */
 typedef struct smla_fwd_cached_params {
     const void* q;              /* bf16 [s_q, h_q, 576] */
     const void* values;

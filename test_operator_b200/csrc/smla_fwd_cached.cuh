@@ -21,10 +21,11 @@
 //   producers  look up pages and scales as well, indices two tiles and pages one tile ahead of the gather; softmax reads (s, log2 s, 1 / s) of
 //              its keys from shared memory.
 // What lives in registers decides: a spill goes to the L2 here, the shared memory leaves the L1 nothing.  So waits are inlined and the split of
-// Q is a call.  4096 queries x 128 heads x top-k 2048, us: two terms by subtraction of the rounded first, indices, pages and scales looked up by
-// every softmax warp, running maximum 2482; packed arithmetic, reference that lags, two producer warps 2250; four 1968 (the two left two of the
+// Q is a call.  On the way here, 4096 queries x 128 heads x top-k 2048, us in short runs: terms in fp32 and indices, pages and scales looked up by every
+// softmax warp, running maximum 2482; packed arithmetic, reference that lags, two producer warps 2250; four 1968 (the two left two of the
 // four sub-partitions' ports idle); pages and scales by the producers 1962, 512 x 64 x 2048 315 -> 301.  Gathers by TMA (tile::gather4, four rows
-// an instruction) 5270: about 65 cycles an instruction.
+// an instruction) 5270: about 65 cycles an instruction.  Now, in calls back to back, under the power cap: 2320 (1.0 PFLOP/s), in short runs 2030; 512 x 64
+// 347 and 299; 3000 x 128 x 512 of short prompts 597 and 578.
 // S [64 heads per CTA x 256 keys] takes five slots of [128 keys x 128 columns] (the fifth half full), O two slots for every 128 keys.
 #pragma once
 #include "smla_cache.cuh"
