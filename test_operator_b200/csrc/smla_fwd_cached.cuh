@@ -567,11 +567,12 @@ smla_fwd_cached_kernel(const KParams p, const CacheView c) {
             float top = ninf;
 #pragma unroll
             for (int i = 0; i < kParts; ++i) top = fmaxf(top, ld_shared_f32(stat + (b * kParts + i) * 256));
-            top -= kTop;
-            if (top > ref + kLag) {      // (first valid tile: ref is -inf, O and the sum are still empty)
+            if (top - ref > kTop + kLag) {       // (first valid tile: ref is -inf, O and the sum are still empty)
+                // Logits of 2^27 bits and more, in steps of 16 and more: no P above what hi + lo holds, wherever the difference is rounded to.
+                const float lower = top - kTop, next = top - lower > kTop + kLag ? top : lower;
                 rescale = ref > ninf;
-                if (rescale) scale_o = ex2_approx(ref - top);
-                ref = top;
+                if (rescale) scale_o = ex2_approx(ref - next);
+                ref = next;
             }
             const float neg = ref == ninf ? 0.f : -ref;
             sum *= scale_o;
